@@ -333,6 +333,114 @@ SA_API int sa_paged_kv_append(int dtype, int64_t B, int64_t Hkv, int64_t D, int6
                               const int64_t* router_strides, void* stream);
 
 /*
+ * Block tables and slot map of a ragged step, from request lengths.  No counterpart in the
+ * reference (nothing there allocates pages); with sa_paged_release, sa_paged_kv_write and
+ * sa_ultrametric_prefix_decode it is the device side of a serving step.
+ *
+ * Request b holds context_lens[b] tokens and gets new_lens[b] more; its rows of the step's flat
+ * token batch are [cu[b], cu[b+1]), cu the running sum of new_lens.  It needs ceil((ctx + new) /
+ * page_size) - ceil(ctx / page_size) pages more, taken in request order from the top of the stack
+ * free_pages[0, num_free): the k-th page taken is free_pages[num_free - 1 - k].  A request is
+ * refused (status bit 2, nothing of it changes, its rows get slot -1) when a length is negative, its
+ * pages exceed max_logical_pages, its rows exceed num_tokens, or it needs pages and the running
+ * sum of pages needed, refused-for-pages requests included, exceeds num_free.
+ *
+ * block_tables      (B, max_logical_pages) int32 with bt_strides, in place: new entries only.
+ * slot_mapping      (num_tokens,) int64 out: page * page_size + row in the page, -1 for refused
+ *                   requests' rows and rows past cu[B].
+ * request_ids       (num_tokens,) int32 out (-1 past cu[B]); positions (num_tokens,) int32 out:
+ *                   position_base + the token's position in its request (0 past cu[B]).
+ * cu_new_lens       (B + 1,) int32 out.
+ * context_lens_out  (B,) int32 out; num_free_out (1,) int32 out: must not alias the inputs, so a
+ *                   call can be repeated.
+ * B <= 16384.  One launch, no synchronisation.
+ */
+SA_API int sa_paged_build_tables(int64_t B, int64_t max_logical_pages, int64_t page_size,
+                                 int64_t num_tokens, const int32_t* context_lens,
+                                 const int32_t* new_lens, int32_t* block_tables,
+                                 const int64_t* bt_strides, const int32_t* free_pages,
+                                 int64_t free_capacity, const int32_t* num_free,
+                                 int64_t position_base, int64_t* slot_mapping,
+                                 int32_t* request_ids, int32_t* positions, int32_t* cu_new_lens,
+                                 int32_t* context_lens_out, int32_t* num_free_out, void* stream);
+
+/*
+ * Return finished requests' pages: for each b with finished[b] != 0, in order, push
+ * block_tables[b][0 .. ceil(context_lens[b] / page_size)) on the stack free_pages (in place above
+ * num_free); context_lens_out[b] = 0, num_free_out = the new height.  A request whose length is
+ * negative or whose pages exceed the table or the stack's capacity keeps them (status bit 2).
+ */
+SA_API int sa_paged_release(int64_t B, int64_t max_logical_pages, int64_t page_size,
+                            const uint8_t* finished, const int32_t* context_lens,
+                            const int32_t* block_tables, const int64_t* bt_strides,
+                            int32_t* free_pages, int64_t free_capacity, const int32_t* num_free,
+                            int32_t* context_lens_out, int32_t* num_free_out, void* stream);
+
+/*
+ * Ragged write into the paged cache: row slot_mapping[t] % page_size of page slot_mapping[t] /
+ * page_size of k_cache / v_cache (P, Hkv, page_size, D) <- k_new / v_new (T, Hkv, D).  Slots < 0
+ * are skipped; slots past the cache are skipped with status bit 2.  When routes (T, H, TD) is
+ * given, router (P, H, TD) of a page <- routes of the last row with a slot in it, which is what one
+ * sa_paged_kv_append per token would leave.  Slots must be distinct and, with routes, the rows of a
+ * page stand together (rows without a slot between them aside).
+ * dtype SA_F32 / SA_F16 / SA_BF16, D contiguous, any other stride; routes/router int32 or int64.
+ */
+SA_API int sa_paged_kv_write(int dtype, int64_t T, int64_t Hkv, int64_t D, int64_t page_size,
+                             int64_t num_pages, const void* k_new, const int64_t* k_new_strides,
+                             const void* v_new, const int64_t* v_new_strides,
+                             const int64_t* slot_mapping, void* k_cache, const int64_t* k_strides,
+                             void* v_cache, const int64_t* v_strides, const void* routes,
+                             int routes_dtype, const int64_t* routes_strides, int64_t H, int64_t TD,
+                             void* router, int router_dtype, const int64_t* router_strides,
+                             void* stream);
+
+/* Bytes of workspace sa_ultrametric_prefix_decode needs for these sizes. */
+SA_API int64_t sa_ultrametric_prefix_decode_workspace_bytes(int dtype, int64_t B, int64_t H,
+                                                            int64_t Hkv, int64_t D,
+                                                            int64_t page_size,
+                                                            int64_t max_prefix_pages,
+                                                            int64_t max_logical_pages);
+
+/*
+ * Routed paged decode of a batch that shares a prefix.  The result is that of
+ * sa_ultrametric_decode over block tables that begin with the prefix's pages, except that the
+ * prefix may end inside its last page (the request's own tokens start on a page of their own); the
+ * prefix's K/V are read once per KV head instead of once per request.
+ *
+ * Request b has the ceil(n / page_size) pages of the prefix (n tokens, n = *prefix_len_dev when
+ * that is not NULL, else prefix_len; pages prefix_pages[0..)) followed by the ceil(context_lens[b] /
+ * page_size) pages of block_tables[b] (own tokens).  Head h attends page l of these when
+ * router[page, h, 0:req_depth] equals q_router[b, h, 0:req_depth], or l == 0 and sink_block, or l is
+ * one of the last local_blocks.  Lengths are cut to their page lists; pages outside [0, num_pages)
+ * are skipped (status bit 2).  A row with nothing to attend gets zeros and lse = -inf.
+ *
+ * dtype             SA_BF16, SA_F16 (tcgen05 path where D % 8 == 0, D <= 128, page_size % 8 == 0
+ *                   and every row of q and the caches is 16-byte aligned) or SA_F32; D <= 256.
+ * q, out            (B, H, D); k_cache, v_cache (P, Hkv, page_size, D); D contiguous.
+ * prefix_pages      (max_prefix_pages,) int32; block_tables (B, max_logical_pages) int32.
+ * router            (P, H, TD), q_router (B, H, TD): SA_I32 or SA_I64 (not read at req_depth 0).
+ * lse               optional fp32 (B, H) out, natural logarithm.
+ * workspace         >= sa_ultrametric_prefix_decode_workspace_bytes() bytes, 256-aligned.
+ */
+SA_API int sa_ultrametric_prefix_decode(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
+                                        int64_t page_size, int64_t num_pages,
+                                        const void* q, const int64_t* q_strides,
+                                        const void* k_cache, const int64_t* k_strides,
+                                        const void* v_cache, const int64_t* v_strides,
+                                        const int32_t* prefix_pages, int64_t max_prefix_pages,
+                                        int64_t prefix_len, const int32_t* prefix_len_dev,
+                                        const int32_t* block_tables, const int64_t* bt_strides,
+                                        int64_t max_logical_pages, const int32_t* context_lens,
+                                        const void* router, int router_dtype,
+                                        const int64_t* router_strides,
+                                        const void* q_router, int q_router_dtype,
+                                        const int64_t* q_router_strides,
+                                        int64_t TD, int64_t req_depth, int64_t local_blocks,
+                                        int sink_block, void* out, const int64_t* out_strides,
+                                        float* lse, void* workspace, int64_t workspace_bytes,
+                                        void* stream);
+
+/*
  * Ternary K/V rows: quantise + pack, and unpack + dequantise.
  * Replaces: src/llama_surgery/surgery.py:15-75 (TernaryQuantize.forward, pack_ternary,
  * unpack_ternary) and the in-kernel unpacking of kernel.py:198-205, 226-232.

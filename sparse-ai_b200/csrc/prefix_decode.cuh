@@ -1,0 +1,58 @@
+// Shared declarations of the shared-prefix decode (general path and entry point in
+// prefix_decode.cu, the tensor-core path in prefix_decode_sm100.cu).
+#pragma once
+
+#include "common.cuh"
+
+namespace sa {
+
+struct PrefixParams {
+  int64_t B, H, Hkv, G, D, page, num_pages;
+  int64_t Lp, L;  // widths of the prefix page list and of the block tables
+  int64_t plen;   // prefix tokens where plen_dev is null
+  const int32_t* plen_dev;
+  int64_t TD, r, local_blocks;
+  int sink;
+  const void* q;
+  int64_t qs[3];
+  const void* kc;
+  int64_t ks[4];
+  const void* vc;
+  int64_t vs[4];
+  const int32_t* ppages;
+  const int32_t* bt;
+  int64_t bts[2];
+  const int32_t* ctx;
+  const void* router;
+  int router_dtype;
+  int64_t rs[3];
+  const void* qrouter;
+  int qrouter_dtype;
+  int64_t qrs[3];
+  void* out;
+  int64_t os[3];
+  float* lse;  // (B, H) natural log, or null
+  unsigned* status;
+};
+
+// Tokens of the prefix and of request b's own pages, within the widths of their page lists.
+__device__ __forceinline__ int64_t prefix_tokens(const PrefixParams& p) {
+  const int64_t n = p.plen_dev ? (int64_t)*p.plen_dev : p.plen;
+  return max((int64_t)0, min(n, p.Lp * p.page));
+}
+__device__ __forceinline__ int64_t own_tokens(const PrefixParams& p, int64_t b) {
+  return max((int64_t)0, min((int64_t)p.ctx[b], p.L * p.page));
+}
+
+// Whether head h of request b attends logical page l (of n), held in physical page phys.
+__device__ __forceinline__ bool page_attended(const PrefixParams& p, int64_t b, int64_t h, int64_t l, int64_t n,
+                                              int64_t phys) {
+  if ((p.sink && l == 0) || l >= n - p.local_blocks) return true;
+  for (int64_t i = 0; i < p.r; ++i)
+    if (load_any_i64(p.router, p.router_dtype, phys * p.rs[0] + h * p.rs[1] + i * p.rs[2]) !=
+        load_any_i64(p.qrouter, p.qrouter_dtype, b * p.qrs[0] + h * p.qrs[1] + i * p.qrs[2]))
+      return false;
+  return true;
+}
+
+}  // namespace sa

@@ -1,5 +1,7 @@
 """B200-native (sm_100a) block-sparse attention with sparse-ai's ``ultrametric`` operator
-surface: routing -> block lists, block-list prefill forward/backward, routed paged decode.
+surface: routing -> block lists, block-list prefill forward/backward, routed paged decode,
+and the operators of a serving step on its paged cache (tables and slots from request lengths,
+ragged K/V writes, decode over a shared prefix).
 
 Only the hot-path modules of the reference package are provided (``block_list``,
 ``kernel``, ``kernel_decode``); the toy models and routers of the reference
@@ -22,6 +24,13 @@ from .kernel import (
     ultrametric_attention_triton,
 )
 from .kernel_decode import ultrametric_decode
+from .kernel_prefix_decode import ultrametric_prefix_decode
+from .paged_tables import (
+    PagedTables,
+    build_paged_tables,
+    paged_kv_write,
+    release_paged_requests,
+)
 
 __all__ = [
     "HAS_TRITON",
@@ -36,4 +45,9 @@ __all__ = [
     "ultrametric_attention_triton",
     "CurriculumSparseAttention",
     "ultrametric_decode",
+    "ultrametric_prefix_decode",
+    "PagedTables",
+    "build_paged_tables",
+    "release_paged_requests",
+    "paged_kv_write",
 ]

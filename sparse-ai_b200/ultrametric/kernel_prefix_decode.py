@@ -1,0 +1,106 @@
+"""Routed paged decode of a batch whose requests share a long prefix, the prefix computed once.
+
+``ultrametric_decode`` (``kernel_decode.py``; sparse-ai's ``src/ultrametric/kernel_decode.py:
+188-247``) reads every request's pages by itself, so a prefix that many requests share -- a system
+prompt, a document that is asked about, several samples of one prompt -- is streamed once per
+request.  ``ultrametric_prefix_decode`` takes the prefix's pages apart from the requests' own:
+the query rows of all requests meet the prefix's keys in one product per KV head, each request
+meets its own pages, and the parts are joined by log-sum-exp.  Routing, sink and local pages act
+on the joined page list, as if the prefix's pages stood first in every block table.
+"""
+
+from __future__ import annotations
+
+from typing import Union
+
+import torch
+
+from . import _native as nat
+
+
+def ultrametric_prefix_decode(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    prefix_pages: torch.Tensor,
+    prefix_len: Union[int, torch.Tensor],
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    router_indices: torch.Tensor,
+    q_router_indices: torch.Tensor,
+    req_depth: int,
+    local_blocks: int = 0,
+    sink_block: bool = False,
+    return_lse: bool = False,
+):
+    """Decode one token per request against a shared prefix and the request's own pages.
+
+    q (B, H, D); k_cache, v_cache (num_pages, Hkv, page_size, D), H % Hkv == 0; prefix_pages (Lp,)
+    int32; ``prefix_len`` tokens of them are valid (an int, or one int32 on the device, which is
+    not read back); block_tables (B, L) int32 and context_lens (B,): each request's own pages and
+    own tokens (0: the prefix alone).  router_indices (num_pages, H, TD), q_router_indices
+    (B, H, TD), req_depth, local_blocks and sink_block as in ``ultrametric_decode``, over the
+    prefix's pages followed by the request's own; req_depth 0 attends every page.
+
+    Returns (B, H, D) in q.dtype, and with ``return_lse`` the (B, H) fp32 natural-log LSE; a row
+    that attends nothing gets zeros and -inf.  fp32, fp16 or bf16; head_dim up to 256.
+    fp16/bf16 with head_dim a multiple of 8 up to 128 and a page size that is a multiple of 8 run
+    on the tensor cores, the rest on the CUDA cores."""
+    if q.dim() != 3:
+        raise ValueError(f"q must be (B, H, D), got {tuple(q.shape)}")
+    B, H, D = q.shape
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"k_cache/v_cache must be (num_pages, Hkv, page_size, D); got "
+                         f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    P, Hkv, page, d2 = k_cache.shape
+    if d2 != D or Hkv == 0 or H % Hkv:
+        raise ValueError("cache head_dim / heads incompatible with q")
+    if not (q.dtype == k_cache.dtype == v_cache.dtype):
+        raise ValueError("q, k_cache, v_cache must share dtype")
+    if prefix_pages.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != B or \
+            tuple(context_lens.shape) != (B,):
+        raise ValueError(f"expected prefix_pages (Lp,), block_tables ({B}, L) and context_lens ({B},); got "
+                         f"{tuple(prefix_pages.shape)}, {tuple(block_tables.shape)}, {tuple(context_lens.shape)}")
+    if router_indices.dim() != 3 or tuple(router_indices.shape[:2]) != (P, H) or \
+            q_router_indices.dim() != 3 or tuple(q_router_indices.shape[:2]) != (B, H) or \
+            q_router_indices.shape[2] < 1 or router_indices.shape[2] != q_router_indices.shape[2]:
+        raise ValueError(f"router_indices must be ({P}, {H}, TD) and q_router_indices ({B}, {H}, TD); got "
+                         f"{tuple(router_indices.shape)}, {tuple(q_router_indices.shape)}")
+    TD = q_router_indices.shape[2]
+    if not 0 <= int(req_depth) <= TD:
+        raise ValueError(f"req_depth must be in [0, {TD}], got {req_depth}")
+    if int(local_blocks) < 0:
+        raise ValueError(f"local_blocks must be >= 0, got {local_blocks}")
+    plen_dev = None
+    if isinstance(prefix_len, torch.Tensor):
+        if prefix_len.dtype != torch.int32 or prefix_len.numel() != 1:
+            raise ValueError(f"prefix_len must be an int or one int32, got {prefix_len.dtype} {tuple(prefix_len.shape)}")
+        plen_dev, plen = prefix_len, 0
+    else:
+        plen = int(prefix_len)
+        if not 0 <= plen <= prefix_pages.shape[0] * page:
+            raise ValueError(f"prefix_len {plen} does not fit {prefix_pages.shape[0]} pages of {page}")
+    nat.require_cuda("ultrametric_prefix_decode", q, k_cache, v_cache, prefix_pages, plen_dev, block_tables,
+                     context_lens, router_indices, q_router_indices)
+    code = nat.float_code(q.dtype)
+    pp = prefix_pages.to(torch.int32).contiguous()
+    bt = block_tables.to(torch.int32)
+    ctx = context_lens.to(torch.int32).contiguous()
+    ri = router_indices if router_indices.dtype in (torch.int32, torch.int64) else router_indices.to(torch.int64)
+    qri = q_router_indices if q_router_indices.dtype in (torch.int32, torch.int64) else q_router_indices.to(torch.int64)
+    kc = k_cache if k_cache.stride(-1) == 1 else k_cache.contiguous()
+    vc = v_cache if v_cache.stride(-1) == 1 else v_cache.contiguous()
+    qq = q if q.stride(-1) == 1 else q.contiguous()
+    out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H), dtype=torch.float32, device=q.device) if return_lse else None
+    Lp, L = pp.shape[0], bt.shape[1]
+    ws_bytes = int(nat.lib().sa_ultrametric_prefix_decode_workspace_bytes(code, B, H, Hkv, D, page, Lp, L))
+    ws = torch.empty(max(ws_bytes, 256), dtype=torch.uint8, device=q.device)
+    nat.check(nat.lib().sa_ultrametric_prefix_decode(
+        code, B, H, Hkv, D, page, P, qq.data_ptr(), nat.strides(qq), kc.data_ptr(), nat.strides(kc),
+        vc.data_ptr(), nat.strides(vc), pp.data_ptr(), Lp, plen, nat.ptr(plen_dev), bt.data_ptr(), nat.strides(bt), L,
+        ctx.data_ptr(), ri.data_ptr(), nat.int_code(ri.dtype), nat.strides(ri), qri.data_ptr(),
+        nat.int_code(qri.dtype), nat.strides(qri), TD, int(req_depth), int(local_blocks), int(bool(sink_block)),
+        out.data_ptr(), nat.strides(out), nat.ptr(lse), ws.data_ptr(), ws.numel(), nat.stream_of(q)),
+        "ultrametric_prefix_decode")
+    return (out, lse) if return_lse else out

@@ -1,0 +1,195 @@
+"""Page allocation, slot maps and ragged K/V writes of a serving step, on the device.
+
+``PagedKVCache`` (``paged.py``) keeps its page allocator on the host and writes one prompt or one
+token per request at a time.  These operators do the same work for a whole ragged step from
+device tensors alone -- request lengths in, tables and slots out -- with no host synchronisation,
+so a step's bookkeeping can follow the previous step's sampling on the device or be captured in a
+CUDA graph:
+
+* ``build_paged_tables``     -> ``sa_paged_build_tables``: pages for the step's new tokens from a
+  stack of free pages, the slot of every new token, positions, row ranges, new lengths;
+* ``release_paged_requests`` -> ``sa_paged_release``: finished requests' pages back on the stack;
+* ``paged_kv_write``         -> ``sa_paged_kv_write``: K/V rows (and the touched pages' routing
+  vectors) into the cache by the slot map.
+
+sparse-ai has no counterpart: its paged decode (``src/ultrametric/kernel_decode.py:188-247``)
+reads such a cache and nothing there writes one.  CUDA tensors only.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _native as nat
+
+
+class PagedTables(NamedTuple):
+    """What ``build_paged_tables`` returns, besides the entries it adds to ``block_tables``.
+
+    slot_mapping:  (num_tokens,) int64, page * page_size + row; -1: no slot.
+    request_ids:   (num_tokens,) int32, the row's request; -1 past the last token.
+    positions:     (num_tokens,) int32, the token's position in its request; 0 past the last.
+    cu_new_lens:   (B + 1,) int32, request b's rows are [cu[b], cu[b + 1]).
+    context_lens:  (B,) int32, lengths after the step.
+    num_free:      (1,) int32, height of the free stack after the step.
+    """
+
+    slot_mapping: torch.Tensor
+    request_ids: torch.Tensor
+    positions: torch.Tensor
+    cu_new_lens: torch.Tensor
+    context_lens: torch.Tensor
+    num_free: torch.Tensor
+
+
+def _int32(name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be int32 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _tables_args(context_lens, block_tables, free_pages, num_free, page_size):
+    if context_lens.dim() != 1 or block_tables.dim() != 2 or free_pages.dim() != 1:
+        raise ValueError("context_lens and free_pages must be 1-d and block_tables 2-d; got "
+                         f"{tuple(context_lens.shape)}, {tuple(free_pages.shape)}, {tuple(block_tables.shape)}")
+    B, L = context_lens.shape[0], block_tables.shape[1]
+    _int32("context_lens", context_lens, (B,))
+    _int32("block_tables", block_tables, (B, L))
+    _int32("free_pages", free_pages, (free_pages.shape[0],))
+    if num_free.dtype != torch.int32 or num_free.numel() != 1:
+        raise ValueError(f"num_free must be one int32, got {num_free.dtype} {tuple(num_free.shape)}")
+    if not free_pages.is_contiguous():
+        raise ValueError("free_pages must be contiguous")
+    if int(page_size) < 1:
+        raise ValueError(f"page_size must be >= 1, got {page_size}")
+    return B, L
+
+
+@torch.no_grad()
+def build_paged_tables(
+    context_lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    free_pages: torch.Tensor,
+    num_free: torch.Tensor,
+    *,
+    page_size: int,
+    num_tokens: int,
+    position_base: int = 0,
+) -> PagedTables:
+    """Pages and slots for ``new_lens[b]`` more tokens of each request.
+
+    context_lens, new_lens  (B,) int32: tokens held, tokens to add (0 for idle requests).
+    block_tables            (B, L) int32, physical page per logical page; the new pages' entries
+                            are written in place, the others are left as they are.
+    free_pages, num_free    (F,) and (1,) int32: a stack of free pages, taken from its top in
+                            request order.  Neither is changed: the new height is returned.
+    num_tokens              rows of the flat token batch (a host number: the sum of ``new_lens``,
+                            or more to keep one shape from step to step).
+    position_base           added to the positions (the length of a shared prefix).
+
+    A request that does not fit (negative length, more than L pages, rows past ``num_tokens``, or
+    no pages left) is refused: its rows get slot -1, its length and table stay, and the device
+    status gets bit 2.  Requests after one that found no pages are refused too if they need any.
+    Nothing is read back to the host."""
+    B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size)
+    _int32("new_lens", new_lens, (B,))
+    if int(num_tokens) < 0:
+        raise ValueError(f"num_tokens must be >= 0, got {num_tokens}")
+    if int(position_base) < 0:
+        raise ValueError(f"position_base must be >= 0, got {position_base}")
+    nat.require_cuda("build_paged_tables", context_lens, new_lens, block_tables, free_pages, num_free)
+    dev, T = context_lens.device, int(num_tokens)
+    ctx, new = context_lens.contiguous(), new_lens.contiguous()
+    out = PagedTables(torch.empty(T, dtype=torch.int64, device=dev), torch.empty(T, dtype=torch.int32, device=dev),
+                      torch.empty(T, dtype=torch.int32, device=dev), torch.empty(B + 1, dtype=torch.int32, device=dev),
+                      torch.empty(B, dtype=torch.int32, device=dev), torch.empty(1, dtype=torch.int32, device=dev))
+    nat.check(nat.lib().sa_paged_build_tables(
+        B, L, int(page_size), T, ctx.data_ptr(), new.data_ptr(), block_tables.data_ptr(), nat.strides(block_tables),
+        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), int(position_base),
+        out.slot_mapping.data_ptr(), out.request_ids.data_ptr(), out.positions.data_ptr(), out.cu_new_lens.data_ptr(),
+        out.context_lens.data_ptr(), out.num_free.data_ptr(), nat.stream_of(ctx)), "build_paged_tables")
+    return out
+
+
+@torch.no_grad()
+def release_paged_requests(
+    finished: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    free_pages: torch.Tensor,
+    num_free: torch.Tensor,
+    *,
+    page_size: int,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Push the pages of every request with ``finished[b]`` ((B,) bool) back on the stack, in
+    request order; returns the new (context_lens, num_free).  ``free_pages`` is written above its
+    old height; the block tables are left as they are."""
+    B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size)
+    if finished.dtype != torch.bool or tuple(finished.shape) != (B,):
+        raise ValueError(f"finished must be bool of shape {(B,)}, got {finished.dtype} {tuple(finished.shape)}")
+    nat.require_cuda("release_paged_requests", finished, context_lens, block_tables, free_pages, num_free)
+    ctx, done = context_lens.contiguous(), finished.contiguous()
+    out_ctx, out_free = torch.empty_like(ctx), torch.empty(1, dtype=torch.int32, device=ctx.device)
+    nat.check(nat.lib().sa_paged_release(
+        B, L, int(page_size), done.data_ptr(), ctx.data_ptr(), block_tables.data_ptr(), nat.strides(block_tables),
+        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), out_ctx.data_ptr(), out_free.data_ptr(),
+        nat.stream_of(ctx)), "release_paged_requests")
+    return out_ctx, out_free
+
+
+@torch.no_grad()
+def paged_kv_write(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    *,
+    routes: Optional[torch.Tensor] = None,
+    router_indices: Optional[torch.Tensor] = None,
+) -> None:
+    """Write T tokens' K/V rows into the paged caches, in place.
+
+    k, v            (T, Hkv, D), any strides with D contiguous (slices of a packed projection).
+    slot_mapping    (T,) int64 as ``build_paged_tables`` makes it: distinct, -1 to skip a row.
+    k_cache, v_cache  (P, Hkv, page_size, D) of k's dtype.
+    routes, router_indices  optional (T, H, TD) and (P, H, TD) int32 or int64: a page that receives
+                    tokens takes the routing vector of the last of them, as one append per token
+                    would leave it (the rows of a page stand together in the batch)."""
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError(f"k and v must be (T, Hkv, D); got {tuple(k.shape)}, {tuple(v.shape)}")
+    T, Hkv, D = k.shape
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+        raise ValueError(f"k_cache/v_cache must be (num_pages, {Hkv}, page_size, {D}); got "
+                         f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+        raise ValueError("k, v, k_cache, v_cache must share dtype")
+    if slot_mapping.dtype != torch.int64 or tuple(slot_mapping.shape) != (T,):
+        raise ValueError(f"slot_mapping must be int64 of shape {(T,)}, got {slot_mapping.dtype} "
+                         f"{tuple(slot_mapping.shape)}")
+    if (routes is None) != (router_indices is None):
+        raise ValueError("routes and router_indices go together")
+    H = TD = 0
+    if routes is not None:
+        if routes.dim() != 3 or router_indices.dim() != 3 or routes.shape[0] != T or \
+                router_indices.shape[0] != k_cache.shape[0] or routes.shape[1:] != router_indices.shape[1:]:
+            raise ValueError(f"routes must be (T, H, TD) and router_indices (num_pages, H, TD); got "
+                             f"{tuple(routes.shape)}, {tuple(router_indices.shape)}")
+        H, TD = routes.shape[1:]
+    if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
+        raise ValueError("the caches' head_dim must be contiguous")
+    nat.require_cuda("paged_kv_write", k, v, slot_mapping, k_cache, v_cache, routes, router_indices)
+    code = nat.float_code(k.dtype)
+    kk = k if k.stride(-1) == 1 else k.contiguous()
+    vv = v if v.stride(-1) == 1 else v.contiguous()
+    slots = slot_mapping.contiguous()
+    nat.check(nat.lib().sa_paged_kv_write(
+        code, T, Hkv, D, k_cache.shape[2], k_cache.shape[0], kk.data_ptr(), nat.strides(kk), vv.data_ptr(),
+        nat.strides(vv), slots.data_ptr(), k_cache.data_ptr(), nat.strides(k_cache), v_cache.data_ptr(),
+        nat.strides(v_cache), nat.ptr(routes), nat.int_code(routes.dtype) if routes is not None else 0,
+        nat.strides(routes) if routes is not None else None, H, TD, nat.ptr(router_indices),
+        nat.int_code(router_indices.dtype) if routes is not None else 0,
+        nat.strides(router_indices) if routes is not None else None, nat.stream_of(k_cache)), "paged_kv_write")

@@ -264,11 +264,13 @@ extern "C" {
 int64_t sa_ultrametric_prefix_decode_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D,
                                                      int64_t page_size, int64_t max_prefix_pages,
                                                      int64_t max_logical_pages) {
-  (void)dtype;
   if (B <= 0 || H <= 0 || Hkv <= 0 || D <= 0 || page_size <= 0 || max_prefix_pages < 0 || max_logical_pages < 0 ||
       H % Hkv)
     return 0;
-  return sa::pd_bytes(B, H, D, sa::pd_split(B, H, Hkv, page_size, max_prefix_pages, max_logical_pages));
+  // alignment decides the path at the call: the larger of the two serves either
+  const int64_t general = sa::pd_bytes(B, H, D, sa::pd_split(B, H, Hkv, page_size, max_prefix_pages, max_logical_pages));
+  if (!sa::prefix_fast_shape(dtype, B, H, Hkv, D, page_size)) return general;
+  return std::max(general, sa::prefix_fast_workspace_bytes(B, H, Hkv, D, page_size, max_prefix_pages, max_logical_pages));
 }
 
 int sa_ultrametric_prefix_decode(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page_size,
@@ -355,6 +357,7 @@ int sa_ultrametric_prefix_decode(int dtype, int64_t B, int64_t H, int64_t Hkv, i
   if (!p.status) return fail(SA_ELAUNCH, std::string("prefix decode: ") + sa_last_error());
   float* part = static_cast<float*>(workspace);
   cudaStream_t s = (cudaStream_t)stream;
+  if (prefix_fast_eligible(p, dtype)) return launch_prefix_fast(p, dtype, workspace, s);
   switch (dtype) {
     case SA_F32: return launch_general<float>(p, part, s);
     case SA_F16: return launch_general<__half>(p, part, s);

@@ -1,0 +1,1104 @@
+// Shared-prefix decode on sm_100a: TMA page loads, tcgen05 products with TMEM accumulators.
+// Semantics in prefix_decode.cu.
+//
+// Per KV head the query rows (request b, head g of the group) of `nb` = 128 / G requests fill one
+// 128-row MMA tile.  Work is cut into key tiles of up to 128 keys (up to kMaxPpt pages), in
+// three segments laid end to end:
+//   pair    prefix tiles against two row tiles at once (2 nb requests): each K/V tile that is
+//           loaded serves 256 rows;
+//   single  prefix tiles against one row tile (the last one where their number is odd);
+//   own     each request's own pages against its G rows, in the same MMA tile shape: 128 - G
+//           rows of the product are unused, but a 128 x 128 tile pair of products takes about 1100
+//           cycles against the 2700 in which one SM's share of HBM delivers the tile's 64 KB.
+// CTA i takes the weighted range [i W / n, (i + 1) W / n) of that line (computed on the device:
+// lengths live there), so every SM gets the same number of tiles whatever the lengths, and a unit
+// (KV head and rows) is cut only where a range ends.  Each (unit, CTA) piece leaves one partial
+// state per row (max, sum, accumulator), which prefix_combine_kernel joins.
+//
+// Persistent kernel, one CTA per SM, 12 warps (register split as in attn_fwd_sm100.cu):
+//   warp 11     scheduler: walks the CTA's range, reads page ids and row masks 32 pages per load,
+//               drops pages that no row attends and pushes tile descriptors into a ring;
+//   warp 8      TMA producer: K and V tiles in turn into one ring of kSlots tiles, Q tiles into two
+//               buffers;
+//   warp 9      MMA issuer.  Jobs (key tile x row tile) alternate between two lanes g = 0, 1, each
+//               with S[g] (fp32, 128 columns) and O[g] in TMEM: for job i it issues
+//               O[g] += P(i-2) V, then S[g] = Q K^T of job i, which may overwrite P(i-2) because
+//               the tensor pipe takes one thread's products in order;
+//   warps 0-7   two softmax warpgroups, one per lane; thread = row: masks by selection, running
+//               maximum (O rescaled in TMEM only when it grows by more than 2^8), exp2, P to TMEM
+//               over S's columns (A operand of the next product), partials to global memory.
+#include <algorithm>
+#include <string>
+#include <type_traits>
+
+#include "prefix_decode.cuh"
+
+namespace sa {
+namespace {
+
+constexpr int kT = 128;          // rows of a row tile, keys of a key tile
+constexpr int kThreads = 384;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kTmemWarp = 10, kSchedWarp = 11;
+constexpr int kLaunchRegs = 168, kCtrlRegs = 72, kSoftmaxRegs = 216;
+static_assert(4 * 32 * kCtrlRegs + 8 * 32 * kSoftmaxRegs <= kThreads * kLaunchRegs,
+              "register split exceeds the launch allocation");
+constexpr int kGroupThreads = 128;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColO = 256;  // S[g] at kColS + 128 g, O[g] at kColO + 128 g
+constexpr int kMaxPpt = 8;                  // pages per key tile
+constexpr uint32_t kMaxSmem = 232448;
+constexpr float kRescaleThreshold = 8.0f;   // log2 units
+constexpr int kMaxHeadWords = 8;            // query heads <= 256 (mask kernel)
+
+// Weights of one key tile in the split of the work over CTAs: a pair tile keeps the tensor and
+// exponential pipes busy about one and a half times as long as any tile's load takes.
+constexpr int kWPair = 3, kWOne = 2;
+
+enum { F_FIRST = 1, F_LAST = 2, F_EMPTY = 4, F_END = 8, F_PAIR = 16, F_OWN = 32 };
+
+struct TileDesc {
+  int flags;
+  int n;     // pages
+  int vr;    // valid keys: rows [0, vr) of the tile
+  int kvh;
+  int b0;    // first request of the row tile(s), or the request of an own item
+  int slot;  // partial slot of the item
+  int t0;    // first row within the page (pages longer than a tile)
+  int pad;
+  int phys[kMaxPpt];
+  uint32_t mask[kMaxPpt][8];  // rows that attend the page: 4 words per row tile
+};
+static_assert(sizeof(TileDesc) == 32 + 32 + 256, "TileDesc");
+
+template <int DT>
+struct Layout {
+  static constexpr uint32_t kTile = kT * DT * 2;  // one K, V or Q tile
+  static constexpr int kSlots = DT == 128 ? 5 : 10;
+  static constexpr int kDescs = DT == 128 ? 4 : 7;
+  static constexpr uint32_t kQ = 0;
+  static constexpr uint32_t kRing = kQ + 2 * kTile;
+  static constexpr uint32_t kDesc = kRing + kSlots * kTile;
+  static constexpr uint32_t kBars = kDesc + kDescs * sizeof(TileDesc);
+  // barriers
+  static constexpr int bFull = 0, bEmpty = bFull + kSlots, bQFull = bEmpty + kSlots, bQEmpty = bQFull + 2,
+                       bSFull = bQEmpty + 2, bPFull = bSFull + 2, bODone = bPFull + 2, bOFree = bODone + 2,
+                       bDFull = bOFree + 2, bDEmpty = bDFull + kDescs, bNum = bDEmpty + kDescs;
+  static constexpr uint32_t kMisc = kBars + bNum * 8;  // tmem slot, scan scratch
+  static constexpr uint32_t kBytes = kMisc + 192;
+  static constexpr uint32_t kAlloc = kBytes + 1024 <= kMaxSmem ? kBytes + 1024 : kMaxSmem;
+  static_assert(kBytes <= kMaxSmem, "prefix decode: shared-memory layout too large");
+};
+
+// Sizes of the split, the same on host and device.
+struct Split {
+  int64_t units[2];  // pair, single: KV heads x groups of row tiles
+  int nb;            // requests per row tile
+  int row_tiles;     // ceil(B / nb)
+  int ppt;           // pages per key tile
+  int sub;           // tiles per page (pages longer than a key tile), else 1
+  int bn;            // TMA box rows
+  int grid;
+};
+
+struct Ws {
+  int* cum;           // [B + 1] own tiles of requests before b (one KV head)
+  uint32_t* mask_p;   // [Hkv][row_tiles][Lp][4]
+  uint32_t* mask_o;   // [B][Hkv][L][WO]
+  float2* ml_p;       // [prefix slots][2][128]
+  float4* acc_p;      // [prefix slots][2][D / 4][128]
+  float2* ml_o;       // [own slots][2][G]
+  float4* acc_o;      // [own slots][2][D / 4][G]
+  int WO;
+};
+
+struct Args {
+  CUtensorMap tm_q, tm_q1, tm_k, tm_v;
+  PrefixParams p;
+  Split s;
+  Ws w;
+  float scale2;
+  int masked;  // row masks are in w (req_depth > 0)
+};
+
+inline Split make_split(int64_t B, int64_t G, int64_t Hkv, int64_t page) {
+  Split s;
+  s.nb = (int)(kT / G);
+  s.row_tiles = (int)((B + s.nb - 1) / s.nb);
+  s.units[0] = Hkv * (s.row_tiles / 2);
+  s.units[1] = Hkv * (s.row_tiles & 1);
+  s.bn = (int)std::min<int64_t>(page, kT);
+  s.sub = (int)((page + kT - 1) / kT);
+  s.ppt = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxPpt, kT / page));
+  s.grid = device_sm_count();
+  return s;
+}
+
+inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+size_t carve(void* base, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t Lp, int64_t L, const Split& s, Ws* w) {
+  char* c = static_cast<char*>(base);
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    char* r = c ? c + o : nullptr;
+    o += al256(bytes);
+    return r;
+  };
+  Ws t;
+  t.WO = G <= 32 ? 1 : 4;
+  const size_t sp = (size_t)(s.units[0] + s.units[1] + s.grid), so = (size_t)(B * Hkv + s.grid);
+  t.cum = reinterpret_cast<int*>(take((size_t)(B + 1) * 4));
+  t.mask_p = reinterpret_cast<uint32_t*>(take((size_t)Hkv * s.row_tiles * Lp * 16));
+  t.mask_o = reinterpret_cast<uint32_t*>(take((size_t)B * Hkv * L * t.WO * 4));
+  t.ml_p = reinterpret_cast<float2*>(take(sp * 2 * kT * 8));
+  t.acc_p = reinterpret_cast<float4*>(take(sp * 2 * kT * D * 4));
+  t.ml_o = reinterpret_cast<float2*>(take(so * 2 * G * 8));
+  t.acc_o = reinterpret_cast<float4*>(take(so * 2 * G * D * 4));
+  if (w) *w = t;
+  return o;
+}
+
+// ---------------------------------------------------------------------------------------
+// the line of work
+// ---------------------------------------------------------------------------------------
+struct Line {
+  int64_t tiles_p;  // key tiles of the prefix
+  int64_t len[3];   // weighted lengths of the segments
+  int64_t W;
+  int n;            // CTAs that get a range
+};
+
+__device__ __forceinline__ int own_tiles(const PrefixParams& p, const Split& s, int64_t b) {
+  const int64_t n = own_tokens(p, b), e = (n + p.page - 1) / p.page * s.sub;
+  return (int)((e + s.ppt - 1) / s.ppt);
+}
+
+__device__ __forceinline__ Line make_line(const PrefixParams& p, const Split& s, int64_t own_total) {
+  Line l;
+  const int64_t n = prefix_tokens(p), e = (n + p.page - 1) / p.page * s.sub;
+  l.tiles_p = (e + s.ppt - 1) / s.ppt;
+  l.len[0] = s.units[0] * l.tiles_p * kWPair;
+  l.len[1] = s.units[1] * l.tiles_p * kWOne;
+  l.len[2] = own_total * p.Hkv * kWOne;
+  l.W = l.len[0] + l.len[1] + l.len[2];
+  // every range spans at least one tile of the heaviest kind, so that a CTA whose range lies inside
+  // a unit holds a piece of it
+  l.n = (int)max((int64_t)1, min((int64_t)s.grid, l.W / kWPair));
+  return l;
+}
+
+__device__ __forceinline__ int64_t range_start(const Line& l, int64_t i) { return i * l.W / l.n; }
+// The CTA whose range holds position x.
+__device__ __forceinline__ int64_t range_of(const Line& l, int64_t x) { return ((x + 1) * l.n - 1) / l.W; }
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
+  uint32_t r;
+  if (bf16)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------
+// row masks (req_depth > 0): which rows attend each page
+// ---------------------------------------------------------------------------------------
+// Warp task: 16 pages against 32 rows (prefix: rows of one mask word; own: 32 heads at a time of one
+// request).  Lane = row: its r levels against the 16 pages' vectors, 16 loads in flight per
+// level; a ballot per page is the page's mask word.  Integer compares of a few MB that sit in L2.
+constexpr int kMaskPages = 16;
+constexpr int kMaskWarps = 4;
+
+template <typename RT>
+__global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const PrefixParams p, const Split s, const Ws w,
+                                                                     int64_t prefix_tasks, int64_t own_tasks) {
+  __shared__ uint32_t s_bits[kMaskWarps][kMaskPages][kMaxHeadWords];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const RT* router = static_cast<const RT*>(p.router);
+  const int64_t pre_pages = (prefix_tokens(p) + p.page - 1) / p.page;
+  const int r = (int)p.r;
+  // bits u = 0..15: whether page u's vector equals the row's on the first r levels
+  auto match = [&](int phys, int64_t b, int64_t h) -> uint32_t {
+    uint32_t bits = (1u << kMaskPages) - 1u;
+    for (int lv = 0; lv < r; ++lv) {
+      const int64_t qv = load_any_i64(p.qrouter, p.qrouter_dtype, b * p.qrs[0] + h * p.qrs[1] + lv * p.qrs[2]);
+      RT rv[kMaskPages];
+#pragma unroll
+      for (int u = 0; u < kMaskPages; ++u)
+        rv[u] = __ldg(router + (int64_t)__shfl_sync(0xffffffffu, phys, u) * p.rs[0] + h * p.rs[1] + lv * p.rs[2]);
+#pragma unroll
+      for (int u = 0; u < kMaskPages; ++u)
+        if ((int64_t)rv[u] != qv) bits &= ~(1u << u);
+    }
+    return bits;
+  };
+  for (int64_t task = (int64_t)blockIdx.x * kMaskWarps + warp; task < prefix_tasks + own_tasks;
+       task += (int64_t)gridDim.x * kMaskWarps) {
+    if (task < prefix_tasks) {
+      int64_t x = task;
+      const int64_t chunks = (p.Lp + kMaskPages - 1) / kMaskPages;
+      const int64_t l0 = (x % chunks) * kMaskPages;
+      x /= chunks;
+      const int word = (int)(x % 4);
+      x /= 4;
+      const int64_t rt = x % s.row_tiles, g = x / s.row_tiles;
+      if (l0 >= pre_pages) continue;
+      const int row = word * 32 + lane;
+      const int64_t b = rt * s.nb + row / p.G, h = g * p.G + row % p.G;
+      const bool live = row < s.nb * p.G && b < p.B;
+      int phys = lane < kMaskPages && l0 + lane < pre_pages ? p.ppages[l0 + lane] : 0;
+      if (phys < 0 || phys >= p.num_pages) phys = 0;  // dropped by the scheduler
+      uint32_t bits = match(phys, live ? b : 0, live ? h : 0);
+      const int64_t n = pre_pages + (live ? (own_tokens(p, b) + p.page - 1) / p.page : 0);
+      for (int u = 0; u < kMaskPages; ++u) {
+        const int64_t l = l0 + u;
+        const bool on = ((bits >> u) & 1u) || (p.sink && l == 0) || l >= n - p.local_blocks;
+        const uint32_t m = __ballot_sync(0xffffffffu, live && on);
+        if (lane == 0 && l < pre_pages) w.mask_p[((g * s.row_tiles + rt) * p.Lp + l) * 4 + word] = m;
+      }
+    } else {
+      int64_t x = task - prefix_tasks;
+      const int64_t chunks = (p.L + kMaskPages - 1) / kMaskPages;
+      const int64_t l0 = (x % chunks) * kMaskPages, b = x / chunks;
+      const int64_t pages = (own_tokens(p, b) + p.page - 1) / p.page;
+      if (l0 >= pages) continue;
+      int phys = lane < kMaskPages && l0 + lane < pages ? p.bt[b * p.bts[0] + (l0 + lane) * p.bts[1]] : 0;
+      if (phys < 0 || phys >= p.num_pages) phys = 0;
+      const int HW = (int)((p.H + 31) / 32);
+      for (int hw = 0; hw < HW; ++hw) {
+        const int64_t h = hw * 32 + lane;
+        const bool live = h < p.H;
+        const uint32_t bits = match(phys, b, live ? h : 0);
+        for (int u = 0; u < kMaskPages; ++u) {
+          const int64_t l = l0 + u;
+          const bool on = ((bits >> u) & 1u) || (p.sink && pre_pages + l == 0) || l >= pages - p.local_blocks;
+          const uint32_t m = __ballot_sync(0xffffffffu, live && on);
+          if (lane == 0) s_bits[warp][u][hw] = m;
+        }
+      }
+      __syncwarp();
+      // each KV head's G bits out of the H
+      const int per = (int)p.Hkv * w.WO;
+      for (int i = lane; i < kMaskPages * per; i += 32) {
+        const int u = i / per, g = (i % per) / w.WO, wd = i % w.WO;
+        if (l0 + u >= pages) continue;
+        const int first = g * (int)p.G + wd * 32, cnt = min(32, (int)p.G - wd * 32);
+        uint32_t m = 0;
+        if (cnt > 0) {
+          const int q = first >> 5, off = first & 31;
+          uint64_t v = s_bits[warp][u][q];
+          if (q + 1 < HW) v |= (uint64_t)s_bits[warp][u][q + 1] << 32;
+          m = (uint32_t)(v >> off);
+          if (cnt < 32) m &= (1u << cnt) - 1u;
+        }
+        w.mask_o[((b * p.Hkv + g) * p.L + l0 + u) * w.WO + wd] = m;
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------------------
+template <int DT, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_constant__ Args a) {
+  using L = Layout<DT>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  {
+    const uint32_t base = smem_u32(smem_raw);
+    uint32_t dyn;
+    asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn));
+    if ((((base + 1023u) & ~1023u) - base) + L::kBytes > dyn) {  // uniform over the CTA
+      if (threadIdx.x == 0) raise_status(a.p.status, kStatusSmemLayout);
+      return;
+    }
+  }
+  unsigned char* sm = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
+  TileDesc* descs = reinterpret_cast<TileDesc*>(sm + L::kDesc);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::kMisc);
+  int* s_warp = reinterpret_cast<int*>(sm + L::kMisc + 16);       // [12] scan
+  int* s_start = reinterpret_cast<int*>(sm + L::kMisc + 80);      // first own request, tiles before it
+  const PrefixParams& p = a.p;
+  const Split& S = a.s;
+  unsigned* st = p.status;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kSlots; ++i) {
+      mbar_init(&bars[L::bFull + i], 1);
+      mbar_init(&bars[L::bEmpty + i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[L::bQFull + i], 1);
+      mbar_init(&bars[L::bQEmpty + i], 1);
+      mbar_init(&bars[L::bSFull + i], 1);
+      mbar_init(&bars[L::bPFull + i], kGroupThreads);
+      mbar_init(&bars[L::bODone + i], 1);
+      mbar_init(&bars[L::bOFree + i], kGroupThreads);
+    }
+    for (int i = 0; i < L::kDescs; ++i) {
+      mbar_init(&bars[L::bDFull + i], 1);
+      mbar_init(&bars[L::bDEmpty + i], 2 + 8);  // producer, MMA warp, 8 softmax warps
+    }
+    fence_mbar_init();
+    prefetch_tmap(&a.tm_k);
+    prefetch_tmap(&a.tm_v);
+    prefetch_tmap(&a.tm_q);
+    prefetch_tmap(&a.tm_q1);
+  }
+  if (warp == kTmemWarp) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+  // ---- own tiles over the requests: every CTA scans them (thread = consecutive requests)
+  const int64_t bper = (p.B + kThreads - 1) / kThreads;
+  const int64_t bfirst = min(p.B, threadIdx.x * bper), bend = min(p.B, bfirst + bper);
+  int mine = 0;
+  for (int64_t b = bfirst; b < bend; ++b) mine += own_tiles(p, S, b);
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  if (threadIdx.x == 0) s_start[0] = (int)p.B;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int before = incl - mine, own_total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int t = s_warp[w];
+    before += w < warp ? t : 0;
+    own_total += t;
+  }
+  const Line line = make_line(p, S, own_total);
+  const bool active = (int)blockIdx.x < line.n && line.W > 0;
+  const int64_t x0 = active ? range_start(line, blockIdx.x) : 0, x1 = active ? range_start(line, blockIdx.x + 1) : 0;
+  const int64_t own_base = line.len[0] + line.len[1];
+  // own tiles [k0, k1) of the CTA; the thread whose requests hold k0 publishes the first one
+  const int64_t k0 = (max((int64_t)0, x0 - own_base) + kWOne - 1) / kWOne;
+  const int64_t k1 = x1 > own_base ? (x1 - own_base + kWOne - 1) / kWOne : 0;
+  {
+    int c = before;
+    for (int64_t b = bfirst; b < bend; ++b) {
+      const int t = own_tiles(p, S, b);
+      if (blockIdx.x == 0) a.w.cum[b] = c;
+      if (k0 >= (int64_t)c * p.Hkv && k0 < (int64_t)(c + t) * p.Hkv) {
+        s_start[0] = (int)b;
+        s_start[1] = c;
+      }
+      c += t;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == kThreads - 1) a.w.cum[p.B] = own_total;
+  }
+  __syncthreads();
+  pdl_trigger();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= kProducerWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
+    if (warp == kSchedWarp) {
+      // ---------------------------------------------------------------- scheduler
+      if (a.masked) pdl_wait();  // the row masks
+      const int ppt = S.ppt, sub = S.sub, bn = S.bn;
+      uint32_t d = 0;  // descriptors pushed
+      bool ok = true;
+      auto acquire = [&]() -> bool {
+        return mbar_wait_warp(&bars[L::bDEmpty + d % L::kDescs], ((d / L::kDescs) & 1) ^ 1, st);
+      };
+      // One item: entries (pages, or 128-key parts of longer pages) [e0, e1) of a page list.
+      auto item = [&](int kind, int64_t kvh, int64_t b0, int64_t slot, const int32_t* ids, int64_t ids_stride,
+                      int64_t tokens, const uint32_t* mask0, const uint32_t* mask1, int mwords, int64_t e0,
+                      int64_t e1) -> bool {
+        const int base_flags = kind == 0 ? F_PAIR : kind == 2 ? F_OWN : 0;
+        if (!acquire()) return false;
+        TileDesc* td = &descs[d % L::kDescs];
+        int cur = 0, vr = 0, t0cur = 0;
+        bool first = true;
+        auto push = [&](int extra) {
+          if (lane == 0) {
+            td->flags = base_flags | (first ? F_FIRST : 0) | extra;
+            td->n = cur;
+            td->vr = vr;
+            td->kvh = (int)kvh;
+            td->b0 = (int)b0;
+            td->slot = (int)slot;
+            td->t0 = t0cur;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[L::bDFull + d % L::kDescs]);
+          ++d;
+          first = false;
+        };
+        for (int64_t eb = e0; eb < e1; eb += 32) {
+          const int64_t e = eb + lane;
+          int phys = -1, valid = 0, t0 = 0;
+          uint4 m0 = make_uint4(~0u, ~0u, ~0u, ~0u), m1 = m0;
+          if (e < e1) {
+            const int64_t l = e / sub;
+            t0 = (int)(e - l * sub) * kT;
+            valid = (int)min((int64_t)kT, min(p.page, tokens - l * p.page) - t0);
+            phys = ids[l * ids_stride];
+            if (a.masked) {
+              if (mwords == 1) {
+                m0 = make_uint4(__ldcg(mask0 + l), 0u, 0u, 0u);
+                m1 = make_uint4(0u, 0u, 0u, 0u);
+              } else {
+                m0 = __ldcg(reinterpret_cast<const uint4*>(mask0) + l);
+                m1 = mask1 ? __ldcg(reinterpret_cast<const uint4*>(mask1) + l) : make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            if (phys < 0 || phys >= p.num_pages) {
+              raise_status(st, kStatusBadIndex);
+              valid = 0;
+            }
+          }
+          const bool live = valid > 0 && ((m0.x | m0.y | m0.z | m0.w) | (m1.x | m1.y | m1.z | m1.w)) != 0u;
+          const unsigned bal = __ballot_sync(0xffffffffu, live);
+          const int total = __popc(bal), rank = __popc(bal & ((1u << lane) - 1u));
+          int done = 0;
+          while (done < total) {
+            if (cur == ppt) {
+              push(0);
+              if (!acquire()) return false;
+              td = &descs[d % L::kDescs];
+              cur = 0;
+            }
+            const int take = min(ppt - cur, total - done);
+            if (live && rank >= done && rank < done + take) {
+              const int j = cur + rank - done;
+              td->phys[j] = phys;
+              *reinterpret_cast<uint4*>(&td->mask[j][0]) = m0;
+              *reinterpret_cast<uint4*>(&td->mask[j][4]) = m1;
+            }
+            // the lane that holds the last page taken
+            const int last = __ffs(__ballot_sync(0xffffffffu, live && rank == done + take - 1)) - 1;
+            cur += take;
+            done += take;
+            vr = (cur - 1) * bn + __shfl_sync(0xffffffffu, valid, last);
+            t0cur = __shfl_sync(0xffffffffu, t0, last);
+          }
+        }
+        push(F_LAST | (cur == 0 ? F_EMPTY : 0));
+        return true;
+      };
+      const int64_t ptok = prefix_tokens(p), pent = (ptok + p.page - 1) / p.page * sub;
+      // prefix segments: units of equal length
+      int64_t base = 0;
+      for (int seg = 0; seg < 2 && ok && active; ++seg) {
+        const int wt = seg == 0 ? kWPair : kWOne;
+        const int64_t lo = max((int64_t)0, x0 - base), hi = min(line.len[seg], x1 - base);
+        if (hi > lo) {
+          const int64_t ka = (lo + wt - 1) / wt, kb = (hi + wt - 1) / wt;
+          for (int64_t k = ka; k < kb && ok;) {
+            const int64_t u = k / line.tiles_p, ta = k - u * line.tiles_p, tb = min(line.tiles_p, ta + (kb - k));
+            const int64_t groups = seg == 0 ? S.row_tiles / 2 : 1;
+            const int64_t kvh = u / groups, rt = seg == 0 ? (u % groups) * 2 : S.row_tiles - 1;
+            const uint32_t* mk = a.w.mask_p + (kvh * S.row_tiles + rt) * p.Lp * 4;
+            ok = item(seg, kvh, rt * S.nb, (seg ? S.units[0] : 0) + u + blockIdx.x, p.ppages, 1, ptok, mk,
+                      seg == 0 ? mk + p.Lp * 4 : nullptr, 4, ta * ppt, min(pent, tb * ppt));
+            k += tb - ta;
+          }
+        }
+        base += line.len[seg];
+      }
+      // own segment
+      if (active && ok && k1 > k0) {
+        int64_t b = s_start[0], c = s_start[1], k = k0;
+        while (k < k1 && b < p.B && ok) {
+          const int64_t tokens = own_tokens(p, b), ent = (tokens + p.page - 1) / p.page * sub;
+          const int64_t t = (ent + ppt - 1) / ppt;
+          while (k < k1 && k < (c + t) * p.Hkv && ok) {
+            const int64_t g = (k - c * p.Hkv) / t, ta = k - c * p.Hkv - g * t, tb = min(t, ta + (k1 - k));
+            ok = item(2, g, b, b * p.Hkv + g + blockIdx.x, p.bt + b * p.bts[0], p.bts[1], tokens,
+                      a.w.mask_o + (b * p.Hkv + g) * p.L * a.w.WO, nullptr, a.w.WO, ta * ppt, min(ent, tb * ppt));
+            k += tb - ta;
+          }
+          c += t;
+          ++b;
+        }
+      }
+      if (ok && acquire()) {
+        if (lane == 0) {
+          descs[d % L::kDescs].flags = F_END;
+          mbar_arrive(&bars[L::bDFull + d % L::kDescs]);
+        }
+      }
+    } else if (warp == kProducerWarp) {
+      // ---------------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        const int dc = (int)((p.D + 63) / 64);  // 64-column chunks
+        const int bn = S.bn;
+        uint32_t d = 0, seq = 0, nq = 0;
+        while (true) {
+          const uint32_t ds = d % L::kDescs;
+          if (!mbar_wait(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+          const TileDesc& td = descs[ds];
+          const int flags = td.flags;
+          if (flags & F_END) break;
+          if (!(flags & F_EMPTY)) {
+            bool ok = true;
+            if (flags & F_FIRST) {
+              const int tiles = flags & F_PAIR ? 2 : 1;
+              for (int i = 0; i < tiles && ok; ++i, ++nq) {
+                const uint32_t qb = nq & 1;
+                if (!(ok = mbar_wait(&bars[L::bQEmpty + qb], ((nq >> 1) & 1) ^ 1, st))) break;
+                unsigned char* dst = sm + L::kQ + qb * L::kTile;
+                const uint32_t rows = (uint32_t)((flags & F_OWN) ? p.G : S.nb * p.G);
+                mbar_arrive_expect_tx(&bars[L::bQFull + qb], rows * 128 * dc);
+                for (int c = 0; c < dc; ++c)
+                  tma_load_4d(dst + c * (kT * 128), (flags & F_OWN) ? &a.tm_q1 : &a.tm_q, &bars[L::bQFull + qb], c * 64,
+                              0, td.kvh, td.b0 + i * S.nb);
+              }
+            }
+            for (int kv = 0; kv < 2 && ok; ++kv, ++seq) {
+              const uint32_t sl = seq % L::kSlots;
+              if (!(ok = mbar_wait(&bars[L::bEmpty + sl], ((seq / L::kSlots) & 1) ^ 1, st))) break;
+              unsigned char* dst = sm + L::kRing + sl * L::kTile;
+              mbar_arrive_expect_tx(&bars[L::bFull + sl], (uint32_t)(td.n * bn * 128 * dc));
+              for (int j = 0; j < td.n; ++j)
+                for (int c = 0; c < dc; ++c)
+                  tma_load_4d(dst + c * (kT * 128) + j * bn * 128, kv ? &a.tm_v : &a.tm_k, &bars[L::bFull + sl], c * 64,
+                              td.t0, td.kvh, td.phys[j]);
+            }
+            if (!ok) break;
+          }
+          mbar_arrive(&bars[L::bDEmpty + ds]);
+          ++d;
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------------- MMA issuer
+      const int dk = (int)((p.D + 15) / 16);  // K steps of Q K^T, and N / 16 of P V
+      const uint32_t id_pv = idesc_f16(kT, dk * 16, BF16, false, true);
+      struct Job {
+        uint32_t tile;  // key tile index: K in ring entry 2 tile, V in 2 tile + 1
+        int lane, vr;
+        bool first, last, fix, rel;
+      };
+      Job j0{}, j1{};  // pending P V products, j0 the older
+      int np = 0;
+      uint32_t d = 0, tile = 0, job = 0, nq = 0, pc0 = 0, pc1 = 0, of0 = 0, of1 = 0;
+      int in_item = 0;  // key tiles of the item so far
+      bool ok = true;
+      auto pv = [&](const Job& j) -> bool {
+        const int g = j.lane;
+        const uint32_t seq = 2 * j.tile + 1, sl = seq % L::kSlots;
+        if (j.first) {  // O[g] has been read by the last item's epilogue
+          if (!mbar_wait_warp(&bars[L::bOFree + g], ((g ? of1 : of0) & 1) ^ 1, st)) return false;
+          if (g) ++of1; else ++of0;
+        }
+        if (!mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) return false;
+        unsigned char* vt = sm + L::kRing + sl * L::kTile;
+        const int n16 = (j.vr + 15) & ~15;
+        if (j.fix && (j.vr & 15)) {
+          // V rows past the valid keys meet P = 0: they must be finite, so they are cleared
+          const int rows = n16 - j.vr, units = rows * (DT / 8);
+          for (int i = lane; i < units; i += 32) {
+            const int rr = j.vr + i / (DT / 8), c = i % (DT / 8);
+            *reinterpret_cast<uint4*>(vt + (c >> 3) * (kT * 128) + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (!mbar_wait_warp(&bars[L::bPFull + g], (g ? pc1 : pc0) & 1, st)) return false;
+        if (g) ++pc1; else ++pc0;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint64_t vd = smem_desc(smem_u32(vt), kT * 128, 1024);
+          const uint32_t d_o = tmem + kColO + g * kT, a_p = tmem + kColS + g * kT;
+          for (int kk = 0; kk < n16 / 16; ++kk)
+            tc_mma_f16_ts(d_o, a_p + kk * 8, desc_add(vd, kk * 16 * 128), id_pv, (!j.first || kk > 0) ? 1u : 0u);
+          if (j.rel) tc_commit(&bars[L::bEmpty + sl]);
+          if (j.last) tc_commit(&bars[L::bODone + g]);
+        }
+        __syncwarp();
+        return true;
+      };
+      while (ok) {
+        const uint32_t ds = d % L::kDescs;
+        if (np == 2) {
+          if (!(ok = pv(j0))) break;
+          j0 = j1;
+          np = 1;
+        }
+        if (!(ok = mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st))) break;
+        const int flags = descs[ds].flags, vr = descs[ds].vr;
+        __syncwarp();
+        if (flags & F_END) break;
+        if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
+        ++d;
+        if (flags & F_EMPTY) {
+          // nothing to multiply: finish what is pending, so that the softmax groups, which wait for
+          // their last item's accumulators, go on releasing descriptors
+          if (np > 0) ok = pv(j0);
+          if (ok && np > 1) ok = pv(j1);
+          np = 0;
+          continue;
+        }
+        const int rts = flags & F_PAIR ? 2 : 1;
+        if (flags & F_FIRST) {
+          in_item = 0;
+          for (int i = 0; i < rts && ok; ++i)
+            ok = mbar_wait_warp(&bars[L::bQFull + ((nq + i) & 1)], ((nq + i) >> 1) & 1, st);
+        }
+        const uint32_t seq = 2 * tile, sl = seq % L::kSlots;
+        ok = ok && mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st);
+        if (!ok) break;
+        const int n16 = (vr + 15) & ~15;
+        const uint32_t id_qk = idesc_f16(kT, n16, BF16, false, false);
+        for (int i = 0; i < rts; ++i, ++job) {
+          const int g = job & 1;
+          if (np == 2) {
+            if (!(ok = pv(j0))) break;
+            j0 = j1;
+            np = 1;
+          }
+          if (lane == 0) {
+            tc_fence_after();
+            const uint64_t qd = smem_desc(smem_u32(sm + L::kQ + ((nq + i) & 1) * L::kTile), 16, 1024);
+            const uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
+            const uint32_t d_s = tmem + kColS + g * kT;
+            for (int kk = 0; kk < dk; ++kk) {
+              const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
+              tc_mma_f16(d_s, desc_add(qd, off), desc_add(kd, off), id_qk, kk > 0 ? 1u : 0u);
+            }
+            tc_commit(&bars[L::bSFull + g]);
+            if (i == rts - 1) tc_commit(&bars[L::bEmpty + sl]);
+            if (flags & F_LAST) tc_commit(&bars[L::bQEmpty + ((nq + i) & 1)]);
+          }
+          __syncwarp();
+          Job j;
+          j.tile = tile;
+          j.lane = g;
+          j.vr = vr;
+          j.fix = i == 0;
+          j.rel = i == rts - 1;
+          // the lane's first product of the item: its first tile's, or, where the lanes take the
+          // tiles in turn, its second tile's
+          j.first = in_item == 0 || (rts == 1 && in_item == 1);
+          j.last = (flags & F_LAST) != 0;
+          if (rts == 1 && j.last && in_item > 0) j0.last = true;  // the other lane's last, still pending
+          if (np == 0) j0 = j; else j1 = j;
+          ++np;
+        }
+        ++tile;
+        ++in_item;
+        if (flags & F_LAST) nq += rts;
+      }
+      if (ok && np > 0) ok = pv(j0);
+      if (ok && np > 1) pv(j1);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------------------------ softmax warpgroups
+    const int grp = warp >> 2, quarter = warp & 3;
+    const int rl = quarter * 32 + lane;  // row of the tile == TMEM lane
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t col_s = kColS + grp * kT, col_o = kColO + grp * kT;
+    const float sc2 = a.scale2;
+    const int G = (int)p.G, D4 = (int)p.D / 4;
+    uint32_t d = 0, job = 0, sc = 0, od = 0;
+    float m_used = -INFINITY, l_sum = 0.f;
+    bool had = false;
+    int sub = 0;        // which of the slot's two states this group writes
+    bool row_ok = false;
+    while (true) {
+      const uint32_t ds = d % L::kDescs;
+      if (!mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+      const TileDesc& td = descs[ds];
+      const int flags = td.flags, vr = td.vr, slot = td.slot, n = td.n;
+      if (flags & F_END) break;
+      const bool pair = flags & F_PAIR, own = flags & F_OWN, empty = flags & F_EMPTY;
+      if (flags & F_FIRST) {
+        sub = pair ? ((int)(job & 1) ^ grp) : grp;
+        m_used = -INFINITY;
+        l_sum = 0.f;
+        had = false;
+        row_ok = own ? rl < G : rl < S.nb * G && (int64_t)td.b0 + (pair ? sub * S.nb : 0) + rl / G < p.B;
+      }
+      const bool mine = !empty && (pair || (int)(job & 1) == grp);
+      // keys in groups of 8 that this row attends (pages are multiples of 8 rows)
+      uint32_t gm = row_ok ? 0xffffu : 0u;
+      if (mine && a.masked) {
+        const int wd = (pair ? sub * 4 : 0) + quarter, g8 = S.bn / 8;
+        gm = 0;
+        for (int j = 0; j < n; ++j)
+          if ((td.mask[j][wd] >> lane) & 1u) gm |= (g8 >= 16 ? 0xffffu : (1u << g8) - 1u) << (j * g8);
+        if (!row_ok) gm = 0;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
+      ++d;
+      if (!empty) job += pair ? 2 : 1;
+      if (mine) {
+        if (!mbar_wait_warp(&bars[L::bSFull + grp], sc & 1, st)) break;
+        ++sc;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, row_ok)) {
+          const int n16 = (vr + 15) & ~15;
+          float s[kT];
+#pragma unroll
+          for (int c = 0; c < kT / 32; ++c) {
+            float chunk[32];
+            if (c * 32 < n16) {
+              tmem_ld32(lane_addr + col_s + c * 32, chunk);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[c * 32 + i] = chunk[i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[c * 32 + i] = -INFINITY;
+            }
+          }
+          tmem_wait_ld();
+          // masked keys by selection (-inf), so that nothing they hold matters
+          if (__any_sync(0xffffffffu, gm != 0xffffu)) {
+#pragma unroll
+            for (int c = 0; c < kT; ++c) s[c] = (gm >> (c >> 3)) & 1u ? s[c] : -INFINITY;
+          }
+          if (vr < kT) {
+#pragma unroll
+            for (int c = 0; c < kT; ++c) s[c] = c < vr ? s[c] : -INFINITY;
+          }
+          float mx[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mx[i] = fmaxf(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+          for (int c = 16; c < kT; c += 2) mx[(c >> 1) & 7] = fmax3(mx[(c >> 1) & 7], s[c], s[c + 1]);
+          const float mraw = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(fmax3(mx[3], mx[4], mx[5]), mx[6], mx[7]));
+          const float mt = mraw * sc2;
+          float m_new = m_used;
+          if (mt > -INFINITY && (m_used == -INFINITY || mt > m_used + kRescaleThreshold)) m_new = mt;
+          const float m_ref = m_new == -INFINITY ? 0.f : m_new;
+          const float alpha = m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_ref);
+          const bool rescale = m_new != m_used && m_used != -INFINITY;
+          const uint64_t scale_x2 = f32x2(sc2, sc2), bias_x2 = f32x2(-m_ref, -m_ref);
+          uint64_t rs[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < kT / 32; ++c) {
+            if (c * 32 < n16) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float e0, e1;
+                f32x2_split(fma_f32x2(f32x2(s[c * 32 + i], s[c * 32 + i + 1]), scale_x2, bias_x2), e0, e1);
+                const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
+                rs[(i >> 1) & 3] = add_f32x2(rs[(i >> 1) & 3], f32x2(p0, p1));
+                pk[i / 2] = pack2(p0, p1, BF16);
+              }
+              tmem_st16(lane_addr + col_s + c * 16, pk);
+            }
+          }
+          // S(i) being complete implies that the lane's last P V is: O[g] may be rescaled here
+          if (had && __any_sync(0xffffffffu, rescale)) {
+            const float f = rescale ? alpha : 1.f;
+            for (int c = 0; c < DT / 32; ++c) {
+              float o[32];
+              tmem_ld32(lane_addr + col_o + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= f;
+              tmem_st32(lane_addr + col_o + c * 32, o);
+            }
+          }
+          tmem_wait_st();
+          float r0, r1;
+          f32x2_split(add_f32x2(add_f32x2(rs[0], rs[1]), add_f32x2(rs[2], rs[3])), r0, r1);
+          l_sum = (m_used == -INFINITY ? 0.f : l_sum * alpha) + (r0 + r1);
+          m_used = m_new;
+        }
+        tc_fence_before();
+        mbar_arrive(&bars[L::bPFull + grp]);
+        had = true;
+      }
+      if (!(flags & F_LAST)) continue;
+      // ---------------------------------------------------------------- the item's partial state
+      const int64_t state = (int64_t)slot * 2 + sub;
+      const int rows = own ? G : kT;
+      float2* ml = (own ? a.w.ml_o : a.w.ml_p) + state * rows;
+      float4* acc = (own ? a.w.acc_o : a.w.acc_p) + state * D4 * rows;
+      if (row_ok) ml[rl] = make_float2(had ? m_used : -INFINITY, l_sum);
+      if (had) {
+        if (!mbar_wait_warp(&bars[L::bODone + grp], od & 1, st)) break;
+        ++od;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, row_ok)) {
+#pragma unroll
+          for (int c = 0; c < DT / 32; ++c) {
+            if (c * 8 < D4) {
+              float o[32];
+              tmem_ld32(lane_addr + col_o + c * 32, o);
+              tmem_wait_ld();
+              if (row_ok && (m_used != -INFINITY || l_sum != 0.f)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (c * 8 + i < D4)
+                    acc[(int64_t)(c * 8 + i) * rows + rl] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&bars[L::bOFree + grp]);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kTmemWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// join of the partial states, one CTA per (request, KV head)
+// ---------------------------------------------------------------------------------------
+constexpr int kCombThreads = 256;
+
+// Row (b, h) by itself, one warp: for rows whose joined state is not finite.  In the tensor-core
+// product a page's V meets every row of the tile, with weight 0 where the row does not attend
+// it; 0 * inf or 0 * NaN would leave a NaN in rows that have nothing to do with the page, so
+// such rows are computed again over their attended keys alone.  Costs tokens x ~100 cycles: only
+// non-finite values get here.
+template <typename T>
+__device__ void exact_row(const PrefixParams& p, int64_t b, int64_t h, float scale2) {
+  const int lane = threadIdx.x & 31;
+  const int64_t g = h / p.G, ptok = prefix_tokens(p), otok = own_tokens(p, b);
+  const int64_t pp = (ptok + p.page - 1) / p.page, n = pp + (otok + p.page - 1) / p.page;
+  const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1];
+  float qv[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) qv[i] = lane + 32 * i < p.D ? to_f32<T>(q[lane + 32 * i]) * scale2 : 0.f;
+  for (int64_t pg = 0; pg < n; ++pg) {
+    const int64_t phys = pg < pp ? p.ppages[pg] : p.bt[b * p.bts[0] + (pg - pp) * p.bts[1]];
+    if (phys < 0 || phys >= p.num_pages || !page_attended(p, b, h, pg, n, phys)) continue;
+    const int64_t valid = min(p.page, pg < pp ? ptok - pg * p.page : otok - (pg - pp) * p.page);
+    for (int64_t t = 0; t < valid; ++t) {
+      const T* k = static_cast<const T*>(p.kc) + phys * p.ks[0] + g * p.ks[1] + t * p.ks[2];
+      const T* v = static_cast<const T*>(p.vc) + phys * p.vs[0] + g * p.vs[1] + t * p.vs[2];
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < p.D) x = fmaf(qv[i], to_f32<T>(k[lane + 32 * i]), x);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      const float mn = fmaxf(m, x), ref = mn == -INFINITY ? 0.f : mn;
+      const float al = exp2f(m - ref), e = exp2f(x - ref);
+      m = mn;
+      l = l * al + e;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < p.D) acc[i] = fmaf(e, to_f32<T>(v[lane + 32 * i]), acc[i] * al);
+    }
+  }
+  T* o = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 32 * i < p.D) o[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] * (1.f / l));
+  if (p.lse && lane == 0) p.lse[b * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const PrefixParams p, const Split s, const Ws w,
+                                                                      float scale2) {
+  __shared__ float4 s_acc[kCombThreads];
+  __shared__ float2 s_ml[kCombThreads];
+  __shared__ unsigned s_bad[4];  // rows (of the group) to compute again
+  const int64_t b = blockIdx.x / p.Hkv, g = blockIdx.x % p.Hkv;
+  const int G = (int)p.G, D4 = (int)p.D / 4, tid = threadIdx.x;
+  if (tid < 4) s_bad[tid] = 0;
+  pdl_wait();
+  const Line line = make_line(p, s, w.cum[p.B]);
+  // pieces of the prefix: row tile rt of KV head g, and of the request's own pages
+  const int rt = (int)(b / s.nb), r0 = (int)(b - (int64_t)rt * s.nb) * G;
+  int64_t sp0 = 0, so0 = 0;  // first slots
+  int npre = 0, nown = 0, sub0 = 0, subs = 1;
+  if (line.W > 0 && line.tiles_p > 0) {
+    const int pairs = s.row_tiles / 2;
+    const bool pair = rt < 2 * pairs;
+    const int64_t u = pair ? g * pairs + rt / 2 : s.units[0] + g;
+    const int64_t x = pair ? u * line.tiles_p * kWPair : line.len[0] + g * line.tiles_p * kWOne;
+    const int64_t i0 = range_of(line, x), i1 = range_of(line, x + (line.tiles_p - 1) * (pair ? kWPair : kWOne));
+    sp0 = u + i0;
+    npre = (int)(i1 - i0 + 1);
+    sub0 = pair ? rt & 1 : 0;
+    subs = pair ? 1 : 2;
+  }
+  const int t_own = w.cum[b + 1] - w.cum[b];
+  if (t_own > 0) {
+    const int64_t x = line.len[0] + line.len[1] + ((int64_t)w.cum[b] * p.Hkv + g * t_own) * kWOne;
+    const int64_t i0 = range_of(line, x), i1 = range_of(line, x + (int64_t)(t_own - 1) * kWOne);
+    so0 = b * p.Hkv + g + i0;
+    nown = (int)(i1 - i0 + 1);
+  }
+  const int total = npre * subs + nown * 2;
+  const int cells = G * D4;                    // float4 outputs of the group
+  const int cpb = min(cells, kCombThreads);    // cells per pass
+  const int CG = kCombThreads / cpb;           // thread groups over the pieces
+  const int cg = tid / cpb, ci = tid % cpb;
+  for (int c0 = 0; c0 < cells; c0 += cpb) {
+    const int cell = c0 + ci;
+    const bool live = cg < CG && cell < cells;
+    const int c4 = live ? cell / G : 0, hh = live ? cell - c4 * G : 0;
+    float M = -INFINITY, Ls = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int NU = 4;
+    for (int k0 = cg; live && k0 < total; k0 += NU * CG) {
+      float2 ml[NU];
+      float4 x[NU];
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const int k = k0 + u * CG;
+        ml[u] = make_float2(-INFINITY, 0.f);
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k < total) {
+          if (k < npre * subs) {
+            const int64_t state = (sp0 + k / subs) * 2 + sub0 + k % subs;
+            ml[u] = __ldcg(w.ml_p + state * kT + r0 + hh);
+            x[u] = __ldcg(w.acc_p + (state * D4 + c4) * kT + r0 + hh);
+          } else {
+            const int64_t state = so0 * 2 + (k - npre * subs);
+            ml[u] = __ldcg(w.ml_o + state * G + hh);
+            x[u] = __ldcg(w.acc_o + (state * D4 + c4) * G + hh);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        if (ml[u].x == -INFINITY && ml[u].y == 0.f) continue;  // nothing attended: acc not written
+        const float mn = fmaxf(M, ml[u].x), ref = mn == -INFINITY ? 0.f : mn;
+        const float so = fast_exp2(M - ref), sn = fast_exp2(ml[u].x - ref);
+        acc.x = acc.x * so + x[u].x * sn;
+        acc.y = acc.y * so + x[u].y * sn;
+        acc.z = acc.z * so + x[u].z * sn;
+        acc.w = acc.w * so + x[u].w * sn;
+        Ls = Ls * so + ml[u].y * sn;
+        M = mn;
+      }
+    }
+    __syncthreads();  // the last pass's shared states are read
+    s_acc[tid] = acc;
+    s_ml[tid] = make_float2(M, Ls);
+    __syncthreads();
+    if (cg == 0 && live) {
+      for (int c = 1; c < CG; ++c) {
+        const float2 ml = s_ml[c * cpb + ci];
+        const float4 x = s_acc[c * cpb + ci];
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+        const float so = fast_exp2(M - ref), sn = fast_exp2(ml.x - ref);
+        acc.x = acc.x * so + x.x * sn;
+        acc.y = acc.y * so + x.y * sn;
+        acc.z = acc.z * so + x.z * sn;
+        acc.w = acc.w * so + x.w * sn;
+        Ls = Ls * so + ml.y * sn;
+        M = mn;
+      }
+      const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+      // an infinite weight or a NaN anywhere makes this sum NaN or infinite
+      if (!(fabsf(acc.x) + fabsf(acc.y) + fabsf(acc.z) + fabsf(acc.w) + fabsf(Ls) < INFINITY))
+        atomicOr(&s_bad[hh >> 5], 1u << (hh & 31));
+      T* o = static_cast<T*>(p.out) + b * p.os[0] + (g * G + hh) * p.os[1] + 4 * c4;
+      o[0] = from_f32<T>(acc.x * inv);
+      o[1] = from_f32<T>(acc.y * inv);
+      o[2] = from_f32<T>(acc.z * inv);
+      o[3] = from_f32<T>(acc.w * inv);
+      if (p.lse && c4 == 0) p.lse[b * p.H + g * G + hh] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
+    }
+  }
+  __syncthreads();
+  for (int hh = tid >> 5; hh < G; hh += kCombThreads / 32)
+    if ((s_bad[hh >> 5] >> (hh & 31)) & 1u) exact_row<T>(p, b, g * G + hh, scale2);
+}
+
+template <int DT, bool BF16>
+int launch_main(const Args& a, bool dependent, cudaStream_t stream) {
+  auto kern = prefix_sm100_kernel<DT, BF16>;
+  // setmaxnreg.inc waits until the registers it asks for are free: launch only when the
+  // per-thread launch allocation is the one the split was sized against
+  static const int regs = [] {
+    cudaFuncAttributes fa{};
+    if (cudaFuncGetAttributes(&fa, prefix_sm100_kernel<DT, BF16>) != cudaSuccess) return -1;
+    return fa.numRegs;
+  }();
+  if (regs != kLaunchRegs)
+    return fail(SA_ELAUNCH, "prefix decode: launch register count " + std::to_string(regs) +
+                                " differs from the register split's " + std::to_string(kLaunchRegs));
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DT>::kAlloc);
+  if (dependent)
+    return launch_dependent(kern, dim3(a.s.grid), dim3(kThreads), Layout<DT>::kAlloc, stream, "prefix_sm100_kernel", a);
+  kern<<<a.s.grid, kThreads, Layout<DT>::kAlloc, stream>>>(a);
+  return check_launch("prefix_sm100_kernel");
+}
+
+}  // namespace
+
+bool prefix_fast_shape(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page) {
+  return (dtype == SA_BF16 || dtype == SA_F16) && D % 8 == 0 && D <= 128 && page % 8 == 0 && H / Hkv <= kT &&
+         H <= 32 * kMaxHeadWords && B * Hkv <= INT32_MAX / 2;
+}
+
+int64_t prefix_fast_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page, int64_t Lp, int64_t L) {
+  return (int64_t)carve(nullptr, B, Hkv, H / Hkv, D, Lp, L, make_split(B, H / Hkv, Hkv, page), nullptr);
+}
+
+bool prefix_fast_eligible(const PrefixParams& p, int dtype) {
+  if (!prefix_fast_shape(dtype, p.B, p.H, p.Hkv, p.D, p.page)) return false;
+  if (p.num_pages < 1 || p.num_pages > INT32_MAX) return false;
+  if (reinterpret_cast<uintptr_t>(p.q) % 16 || reinterpret_cast<uintptr_t>(p.kc) % 16 ||
+      reinterpret_cast<uintptr_t>(p.vc) % 16)
+    return false;
+  for (int i = 0; i < 2; ++i)
+    if (p.qs[i] % 8) return false;
+  for (int i = 0; i < 3; ++i)
+    if (p.ks[i] % 8 || p.vs[i] % 8) return false;
+  return true;
+}
+
+int launch_prefix_fast(const PrefixParams& p, int dtype, void* workspace, cudaStream_t stream) {
+  Args a{};
+  a.p = p;
+  a.s = make_split(p.B, p.G, p.Hkv, p.page);
+  carve(workspace, p.B, p.Hkv, p.G, p.D, p.Lp, p.L, a.s, &a.w);
+  a.scale2 = (1.0f / sqrtf((float)p.D)) * kLog2e;
+  a.masked = p.r > 0;
+  // query rows as (D, G, KV head, request): a box of nb requests is one row tile
+  const int64_t qst[4] = {p.qs[0], p.G * p.qs[1], p.qs[1], 1};
+  int rc = make_tmap_4d(&a.tm_q, p.q, dtype, p.B, p.Hkv, p.G, p.D, qst, 64, (uint32_t)p.G, (uint32_t)a.s.nb);
+  if (!rc) rc = make_tmap_4d(&a.tm_q1, p.q, dtype, p.B, p.Hkv, p.G, p.D, qst, 64, (uint32_t)p.G);
+  if (!rc) rc = make_tmap_4d(&a.tm_k, p.kc, dtype, p.num_pages, p.Hkv, p.page, p.D, p.ks, 64, (uint32_t)a.s.bn);
+  if (!rc) rc = make_tmap_4d(&a.tm_v, p.vc, dtype, p.num_pages, p.Hkv, p.page, p.D, p.vs, 64, (uint32_t)a.s.bn);
+  if (rc) return fail(SA_ELAUNCH, std::string("prefix decode tensor maps: ") + sa_last_error());
+  if (a.masked) {
+    const int64_t pt = p.Hkv * a.s.row_tiles * 4 * ((p.Lp + kMaskPages - 1) / kMaskPages);
+    const int64_t ot = p.B * ((p.L + kMaskPages - 1) / kMaskPages);
+    const int grid = (int)std::max<int64_t>(
+        1, std::min<int64_t>((pt + ot + kMaskWarps - 1) / kMaskWarps, (int64_t)device_sm_count() * 8));
+    if (p.router_dtype == SA_I64)
+      prefix_mask_kernel<int64_t><<<grid, kMaskWarps * 32, 0, stream>>>(p, a.s, a.w, pt, ot);
+    else
+      prefix_mask_kernel<int32_t><<<grid, kMaskWarps * 32, 0, stream>>>(p, a.s, a.w, pt, ot);
+    if ((rc = check_launch("prefix_mask_kernel"))) return rc;
+  }
+  const bool bf = dtype == SA_BF16;
+  if (p.D <= 64)
+    rc = bf ? launch_main<64, true>(a, a.masked, stream) : launch_main<64, false>(a, a.masked, stream);
+  else
+    rc = bf ? launch_main<128, true>(a, a.masked, stream) : launch_main<128, false>(a, a.masked, stream);
+  if (rc) return rc;
+  const dim3 grid((unsigned)(p.B * p.Hkv)), block(kCombThreads);
+  if (bf)
+    return launch_dependent(prefix_combine_kernel<__nv_bfloat16>, grid, block, 0, stream, "prefix_combine_kernel", p, a.s,
+                            a.w, a.scale2);
+  return launch_dependent(prefix_combine_kernel<__half>, grid, block, 0, stream, "prefix_combine_kernel", p, a.s, a.w,
+                          a.scale2);
+}
+
+}  // namespace sa

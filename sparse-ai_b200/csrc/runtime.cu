@@ -146,7 +146,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 int make_tmap_4d(CUtensorMap* map, const void* base, int dtype, int64_t Z, int64_t Hh, int64_t N,
-                 int64_t D, const int64_t* strides, uint32_t box_d, uint32_t box_n) {
+                 int64_t D, const int64_t* strides, uint32_t box_d, uint32_t box_n, uint32_t box_z) {
   auto fn = encode_fn();
   if (!fn) return fail(SA_ELAUNCH, "cuTensorMapEncodeTiled is unavailable");
   const int64_t esz = dtype == SA_F32 ? 4 : 2;
@@ -163,7 +163,7 @@ int make_tmap_4d(CUtensorMap* map, const void* base, int dtype, int64_t Z, int64
   if (N == 1) gstr[0] = (cuuint64_t)(D * esz);
   if (Hh == 1) gstr[1] = gstr[0] * (cuuint64_t)N;
   if (Z == 1) gstr[2] = gstr[1] * (cuuint64_t)Hh;
-  cuuint32_t box[4] = {box_d, box_n, 1, 1};
+  cuuint32_t box[4] = {box_d, box_n, 1, box_z};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUtensorMapDataType dt = dtype == SA_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                            : dtype == SA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16

@@ -89,15 +89,18 @@ struct Layout {
   static_assert(kBytes <= kMaxSmem, "prefix decode: shared-memory layout too large");
 };
 
-// Sizes of the split, the same on host and device.
+// Sizes of the split, the same on host and device.  32-bit throughout the kernels: the launcher
+// sends anything larger to the general path.
 struct Split {
-  int64_t units[2];  // pair, single: KV heads x groups of row tiles
-  int nb;            // requests per row tile
-  int row_tiles;     // ceil(B / nb)
-  int ppt;           // pages per key tile
-  int sub;           // tiles per page (pages longer than a key tile), else 1
-  int bn;            // TMA box rows
+  int units[2];   // pair, single: KV heads x groups of row tiles
+  int nb;         // requests per row tile
+  int row_tiles;  // ceil(B / nb)
+  int ppt;        // pages per key tile
+  int sub;        // tiles per page (pages longer than a key tile), else 1
+  int span;       // keys per `sub` tiles: ppt pages, or one long page
+  int bn;         // TMA box rows
   int grid;
+  int B, G, Hkv, page, Lp, L, D;
 };
 
 struct Ws {
@@ -113,29 +116,44 @@ struct Ws {
 
 struct Args {
   CUtensorMap tm_q, tm_q1, tm_k, tm_v;
-  PrefixParams p;
   Split s;
   Ws w;
+  const int32_t* ppages;
+  const int32_t* bt;
+  int64_t bts0, bts1;
+  const int32_t* ctx;
+  const int32_t* plen_dev;
+  int plen, num_pages;
   float scale2;
   int masked;  // row masks are in w (req_depth > 0)
+  unsigned* status;
 };
 
-inline Split make_split(int64_t B, int64_t G, int64_t Hkv, int64_t page) {
+inline Split make_split(int64_t B, int64_t G, int64_t Hkv, int64_t page, int64_t Lp, int64_t L, int64_t D) {
   Split s;
   s.nb = (int)(kT / G);
   s.row_tiles = (int)((B + s.nb - 1) / s.nb);
-  s.units[0] = Hkv * (s.row_tiles / 2);
-  s.units[1] = Hkv * (s.row_tiles & 1);
+  s.units[0] = (int)(Hkv * (s.row_tiles / 2));
+  s.units[1] = (int)(Hkv * (s.row_tiles & 1));
   s.bn = (int)std::min<int64_t>(page, kT);
   s.sub = (int)((page + kT - 1) / kT);
   s.ppt = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxPpt, kT / page));
+  s.span = (int)page * s.ppt;
   s.grid = device_sm_count();
+  s.B = (int)B;
+  s.G = (int)G;
+  s.Hkv = (int)Hkv;
+  s.page = (int)page;
+  s.Lp = (int)Lp;
+  s.L = (int)L;
+  s.D = (int)D;
   return s;
 }
 
 inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-size_t carve(void* base, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t Lp, int64_t L, const Split& s, Ws* w) {
+size_t carve(void* base, const Split& s, Ws* w) {
+  const int64_t B = s.B, Hkv = s.Hkv, G = s.G, D = s.D, Lp = s.Lp, L = s.L;
   char* c = static_cast<char*>(base);
   size_t o = 0;
   auto take = [&](size_t bytes) {
@@ -145,7 +163,7 @@ size_t carve(void* base, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t L
   };
   Ws t;
   t.WO = G <= 32 ? 1 : 4;
-  const size_t sp = (size_t)(s.units[0] + s.units[1] + s.grid), so = (size_t)(B * Hkv + s.grid);
+  const size_t sp = (size_t)s.units[0] + s.units[1] + s.grid, so = (size_t)(B * Hkv + s.grid);
   t.cum = reinterpret_cast<int*>(take((size_t)(B + 1) * 4));
   t.mask_p = reinterpret_cast<uint32_t*>(take((size_t)Hkv * s.row_tiles * Lp * 16));
   t.mask_o = reinterpret_cast<uint32_t*>(take((size_t)B * Hkv * L * t.WO * 4));
@@ -161,24 +179,28 @@ size_t carve(void* base, int64_t B, int64_t Hkv, int64_t G, int64_t D, int64_t L
 // the line of work
 // ---------------------------------------------------------------------------------------
 struct Line {
-  int64_t tiles_p;  // key tiles of the prefix
+  int tiles_p;      // key tiles of the prefix
   int64_t len[3];   // weighted lengths of the segments
   int64_t W;
   int n;            // CTAs that get a range
 };
 
-__device__ __forceinline__ int own_tiles(const PrefixParams& p, const Split& s, int64_t b) {
-  const int64_t n = own_tokens(p, b), e = (n + p.page - 1) / p.page * s.sub;
-  return (int)((e + s.ppt - 1) / s.ppt);
+// Valid tokens of a length within a list of `width` pages.
+__device__ __forceinline__ int tokens_in(int n, int width, int page) { return max(0, min(n, width * page)); }
+__device__ __forceinline__ int pre_tokens(const Split& s, const int32_t* dev, int plen) {
+  return tokens_in(dev ? *dev : plen, s.Lp, s.page);
+}
+// Key tiles of n tokens.
+__device__ __forceinline__ int tiles_of(const Split& s, int n) {
+  return (int)(((unsigned)n + (unsigned)s.span - 1u) / (unsigned)s.span) * s.sub;
 }
 
-__device__ __forceinline__ Line make_line(const PrefixParams& p, const Split& s, int64_t own_total) {
+__device__ __forceinline__ Line make_line(const Split& s, int prefix_tokens, int own_total) {
   Line l;
-  const int64_t n = prefix_tokens(p), e = (n + p.page - 1) / p.page * s.sub;
-  l.tiles_p = (e + s.ppt - 1) / s.ppt;
-  l.len[0] = s.units[0] * l.tiles_p * kWPair;
-  l.len[1] = s.units[1] * l.tiles_p * kWOne;
-  l.len[2] = own_total * p.Hkv * kWOne;
+  l.tiles_p = tiles_of(s, prefix_tokens);
+  l.len[0] = (int64_t)s.units[0] * l.tiles_p * kWPair;
+  l.len[1] = (int64_t)s.units[1] * l.tiles_p * kWOne;
+  l.len[2] = (int64_t)own_total * s.Hkv * kWOne;
   l.W = l.len[0] + l.len[1] + l.len[2];
   // every range spans at least one tile of the heaviest kind, so that a CTA whose range lies inside
   // a unit holds a piece of it
@@ -186,9 +208,9 @@ __device__ __forceinline__ Line make_line(const PrefixParams& p, const Split& s,
   return l;
 }
 
-__device__ __forceinline__ int64_t range_start(const Line& l, int64_t i) { return i * l.W / l.n; }
+__device__ __forceinline__ int64_t range_start(const Line& l, int i) { return i * l.W / l.n; }
 // The CTA whose range holds position x.
-__device__ __forceinline__ int64_t range_of(const Line& l, int64_t x) { return ((x + 1) * l.n - 1) / l.W; }
+__device__ __forceinline__ int range_of(const Line& l, int64_t x) { return (int)(((x + 1) * l.n - 1) / l.W); }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
   uint32_t r;
@@ -310,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     uint32_t dyn;
     asm("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn));
     if ((((base + 1023u) & ~1023u) - base) + L::kBytes > dyn) {  // uniform over the CTA
-      if (threadIdx.x == 0) raise_status(a.p.status, kStatusSmemLayout);
+      if (threadIdx.x == 0) raise_status(a.status, kStatusSmemLayout);
       return;
     }
   }
@@ -321,9 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::kMisc);
   int* s_warp = reinterpret_cast<int*>(sm + L::kMisc + 16);       // [12] scan
   int* s_start = reinterpret_cast<int*>(sm + L::kMisc + 80);      // first own request, tiles before it
-  const PrefixParams& p = a.p;
   const Split& S = a.s;
-  unsigned* st = p.status;
+  unsigned* st = a.status;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -354,10 +375,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     tmem_relinquish();
   }
   // ---- own tiles over the requests: every CTA scans them (thread = consecutive requests)
-  const int64_t bper = (p.B + kThreads - 1) / kThreads;
-  const int64_t bfirst = min(p.B, threadIdx.x * bper), bend = min(p.B, bfirst + bper);
+  const int bper = (S.B + kThreads - 1) / kThreads;
+  const int bfirst = min(S.B, (int)threadIdx.x * bper), bend = min(S.B, bfirst + bper);
   int mine = 0;
-  for (int64_t b = bfirst; b < bend; ++b) mine += own_tiles(p, S, b);
+#pragma unroll 1
+  for (int b = bfirst; b < bend; ++b) mine += tiles_of(S, tokens_in(a.ctx[b], S.L, S.page));
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -365,7 +387,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     if (lane >= o) incl += y;
   }
   if (lane == 31) s_warp[warp] = incl;
-  if (threadIdx.x == 0) s_start[0] = (int)p.B;
+  if (threadIdx.x == 0) s_start[0] = S.B;
+  const int ptok = pre_tokens(S, a.plen_dev, a.plen);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -376,25 +399,30 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     before += w < warp ? t : 0;
     own_total += t;
   }
-  const Line line = make_line(p, S, own_total);
+  const Line line = make_line(S, ptok, own_total);
   const bool active = (int)blockIdx.x < line.n && line.W > 0;
   const int64_t x0 = active ? range_start(line, blockIdx.x) : 0, x1 = active ? range_start(line, blockIdx.x + 1) : 0;
+  // the CTA's tiles [lo, hi) of a segment that starts at `base` and whose tiles weigh wt
+  auto seg_lo = [&](int64_t base, int wt) { return (int)((max((int64_t)0, x0 - base) + wt - 1) / wt); };
+  auto seg_hi = [&](int64_t base, int64_t len, int wt) {
+    return (int)((max((int64_t)0, min(len, x1 - base)) + wt - 1) / wt);
+  };
   const int64_t own_base = line.len[0] + line.len[1];
   // own tiles [k0, k1) of the CTA; the thread whose requests hold k0 publishes the first one
-  const int64_t k0 = (max((int64_t)0, x0 - own_base) + kWOne - 1) / kWOne;
-  const int64_t k1 = x1 > own_base ? (x1 - own_base + kWOne - 1) / kWOne : 0;
+  const int k0 = seg_lo(own_base, kWOne), k1 = seg_hi(own_base, line.len[2], kWOne);
   {
     int c = before;
-    for (int64_t b = bfirst; b < bend; ++b) {
-      const int t = own_tiles(p, S, b);
+#pragma unroll 1
+    for (int b = bfirst; b < bend; ++b) {
+      const int t = tiles_of(S, tokens_in(a.ctx[b], S.L, S.page));
       if (blockIdx.x == 0) a.w.cum[b] = c;
-      if (k0 >= (int64_t)c * p.Hkv && k0 < (int64_t)(c + t) * p.Hkv) {
-        s_start[0] = (int)b;
+      if (k0 >= c * S.Hkv && k0 < (c + t) * S.Hkv) {
+        s_start[0] = b;
         s_start[1] = c;
       }
       c += t;
     }
-    if (blockIdx.x == 0 && threadIdx.x == kThreads - 1) a.w.cum[p.B] = own_total;
+    if (blockIdx.x == 0 && threadIdx.x == kThreads - 1) a.w.cum[S.B] = own_total;
   }
   __syncthreads();
   pdl_trigger();
@@ -408,67 +436,111 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       const int ppt = S.ppt, sub = S.sub, bn = S.bn;
       uint32_t d = 0;  // descriptors pushed
       bool ok = true;
-      auto acquire = [&]() -> bool {
-        return mbar_wait_warp(&bars[L::bDEmpty + d % L::kDescs], ((d / L::kDescs) & 1) ^ 1, st);
-      };
-      // One item: entries (pages, or 128-key parts of longer pages) [e0, e1) of a page list.
-      auto item = [&](int kind, int64_t kvh, int64_t b0, int64_t slot, const int32_t* ids, int64_t ids_stride,
-                      int64_t tokens, const uint32_t* mask0, const uint32_t* mask1, int mwords, int64_t e0,
-                      int64_t e1) -> bool {
-        const int base_flags = kind == 0 ? F_PAIR : kind == 2 ? F_OWN : 0;
-        if (!acquire()) return false;
-        TileDesc* td = &descs[d % L::kDescs];
-        int cur = 0, vr = 0, t0cur = 0;
-        bool first = true;
-        auto push = [&](int extra) {
-          if (lane == 0) {
-            td->flags = base_flags | (first ? F_FIRST : 0) | extra;
-            td->n = cur;
-            td->vr = vr;
-            td->kvh = (int)kvh;
-            td->b0 = (int)b0;
-            td->slot = (int)slot;
-            td->t0 = t0cur;
+      // position in the line: segment (pair, single, own), tiles [k, hi) of it, and in the own
+      // segment the request b with c tiles (of one KV head) before it and t of its own
+      int seg = -1, k = 0, hi = 0, b = 0, c = 0, t = 0, own_tok = 0;
+      while (ok) {
+        while (k >= hi && seg < 3) {  // the next segment with work
+          ++seg;
+          if (!active || seg > 2) {
+            seg = 3;
+          } else if (seg == 2) {
+            k = k0;
+            hi = k1;
+            b = s_start[0];
+            c = s_start[1];
+            if (k < hi) {
+              own_tok = tokens_in(a.ctx[b], S.L, S.page);
+              t = tiles_of(S, own_tok);
+            }
+          } else {
+            const int64_t base = seg ? line.len[0] : 0, len = seg ? line.len[1] : line.len[0];
+            const int wt = seg ? kWOne : kWPair;
+            k = seg_lo(base, wt);
+            hi = seg_hi(base, len, wt);
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[L::bDFull + d % L::kDescs]);
-          ++d;
-          first = false;
-        };
-        for (int64_t eb = e0; eb < e1; eb += 32) {
-          const int64_t e = eb + lane;
-          int phys = -1, valid = 0, t0 = 0;
-          uint4 m0 = make_uint4(~0u, ~0u, ~0u, ~0u), m1 = m0;
-          if (e < e1) {
-            const int64_t l = e / sub;
-            t0 = (int)(e - l * sub) * kT;
-            valid = (int)min((int64_t)kT, min(p.page, tokens - l * p.page) - t0);
-            phys = ids[l * ids_stride];
-            if (a.masked) {
-              if (mwords == 1) {
-                m0 = make_uint4(__ldcg(mask0 + l), 0u, 0u, 0u);
-                m1 = make_uint4(0u, 0u, 0u, 0u);
-              } else {
-                m0 = __ldcg(reinterpret_cast<const uint4*>(mask0) + l);
-                m1 = mask1 ? __ldcg(reinterpret_cast<const uint4*>(mask1) + l) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        // ---- the next item: tiles [ta, tb) of one unit
+        int flags = F_END, kvh = 0, b0 = 0, slot = 0, ta = 0, tb = 0, tokens = 0, mwords = 4;
+        const int32_t* ids = a.ppages;
+        int64_t ids_stride = 1;
+        const uint32_t *mask0 = nullptr, *mask1 = nullptr;
+        if (seg < 2) {
+          const int u = k / line.tiles_p, groups = seg == 0 ? S.row_tiles / 2 : 1;
+          ta = k - u * line.tiles_p;
+          tb = min(line.tiles_p, ta + hi - k);
+          kvh = u / groups;
+          const int rt = seg == 0 ? (u - kvh * groups) * 2 : S.row_tiles - 1;
+          flags = seg == 0 ? F_PAIR : 0;
+          b0 = rt * S.nb;
+          slot = (seg ? S.units[0] : 0) + u + (int)blockIdx.x;
+          tokens = ptok;
+          mask0 = a.w.mask_p + ((int64_t)kvh * S.row_tiles + rt) * S.Lp * 4;
+          if (seg == 0) mask1 = mask0 + (int64_t)S.Lp * 4;
+        } else if (seg == 2) {
+          while (k >= (c + t) * S.Hkv) {  // hi > k: there is such a request
+            c += t;
+            own_tok = tokens_in(a.ctx[++b], S.L, S.page);
+            t = tiles_of(S, own_tok);
+          }
+          const int r = k - c * S.Hkv;
+          kvh = r / t;
+          ta = r - kvh * t;
+          tb = min(t, ta + hi - k);
+          flags = F_OWN;
+          b0 = b;
+          slot = b * S.Hkv + kvh + (int)blockIdx.x;
+          tokens = own_tok;
+          ids = a.bt + b * a.bts0;
+          ids_stride = a.bts1;
+          mwords = a.w.WO;
+          mask0 = a.w.mask_o + ((int64_t)b * S.Hkv + kvh) * S.L * mwords;
+        }
+        k += tb - ta;
+        // ---- its entries: pages, or 128-key parts of longer pages
+        TileDesc* td;
+        int cur = 0, vr = 0, t0cur = 0, more = 1;
+        int eb = ta * ppt, e1 = tb * ppt;
+        int first = F_FIRST, total = 0, done = 0, phys = 0, valid = 0, t0 = 0, rank = 0;
+        bool live = false;
+        uint4 m0, m1;
+        while (more) {  // one descriptor per turn
+          td = &descs[d % L::kDescs];
+          if (!(ok = mbar_wait_warp(&bars[L::bDEmpty + d % L::kDescs], ((d / L::kDescs) & 1) ^ 1, st))) break;
+          cur = 0;
+          while (true) {
+            if (done == total) {  // the next 32 entries
+              if (eb >= e1) break;
+              const int e = eb + lane, l = sub == 1 ? e : e / sub;
+              t0 = sub == 1 ? 0 : (e - l * sub) * kT;
+              valid = e < e1 ? min(kT, min(S.page, tokens - l * S.page) - t0) : 0;
+              phys = -1;
+              m0 = m1 = make_uint4(~0u, ~0u, ~0u, ~0u);
+              if (valid > 0) {
+                phys = ids[l * ids_stride];
+                if (a.masked) {
+                  m1 = make_uint4(0u, 0u, 0u, 0u);
+                  if (mwords == 1) {
+                    m0 = make_uint4(__ldcg(mask0 + l), 0u, 0u, 0u);
+                  } else {
+                    m0 = __ldcg(reinterpret_cast<const uint4*>(mask0) + l);
+                    if (mask1) m1 = __ldcg(reinterpret_cast<const uint4*>(mask1) + l);
+                  }
+                }
+                if (phys < 0 || phys >= a.num_pages) {
+                  raise_status(st, kStatusBadIndex);
+                  valid = 0;
+                }
               }
+              live = valid > 0 && ((m0.x | m0.y | m0.z | m0.w) | (m1.x | m1.y | m1.z | m1.w)) != 0u;
+              const unsigned bal = __ballot_sync(0xffffffffu, live);
+              total = __popc(bal);
+              rank = __popc(bal & ((1u << lane) - 1u));
+              done = 0;
+              eb += 32;
+              continue;
             }
-            if (phys < 0 || phys >= p.num_pages) {
-              raise_status(st, kStatusBadIndex);
-              valid = 0;
-            }
-          }
-          const bool live = valid > 0 && ((m0.x | m0.y | m0.z | m0.w) | (m1.x | m1.y | m1.z | m1.w)) != 0u;
-          const unsigned bal = __ballot_sync(0xffffffffu, live);
-          const int total = __popc(bal), rank = __popc(bal & ((1u << lane) - 1u));
-          int done = 0;
-          while (done < total) {
-            if (cur == ppt) {
-              push(0);
-              if (!acquire()) return false;
-              td = &descs[d % L::kDescs];
-              cur = 0;
-            }
+            if (cur == ppt) break;
             const int take = min(ppt - cur, total - done);
             if (live && rank >= done && rank < done + take) {
               const int j = cur + rank - done;
@@ -476,223 +548,200 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
               *reinterpret_cast<uint4*>(&td->mask[j][0]) = m0;
               *reinterpret_cast<uint4*>(&td->mask[j][4]) = m1;
             }
-            // the lane that holds the last page taken
-            const int last = __ffs(__ballot_sync(0xffffffffu, live && rank == done + take - 1)) - 1;
             cur += take;
             done += take;
+            // the lane that holds the last page taken
+            const int last = __ffs(__ballot_sync(0xffffffffu, live && rank == done - 1)) - 1;
             vr = (cur - 1) * bn + __shfl_sync(0xffffffffu, valid, last);
             t0cur = __shfl_sync(0xffffffffu, t0, last);
           }
-        }
-        push(F_LAST | (cur == 0 ? F_EMPTY : 0));
-        return true;
-      };
-      const int64_t ptok = prefix_tokens(p), pent = (ptok + p.page - 1) / p.page * sub;
-      // prefix segments: units of equal length
-      int64_t base = 0;
-      for (int seg = 0; seg < 2 && ok && active; ++seg) {
-        const int wt = seg == 0 ? kWPair : kWOne;
-        const int64_t lo = max((int64_t)0, x0 - base), hi = min(line.len[seg], x1 - base);
-        if (hi > lo) {
-          const int64_t ka = (lo + wt - 1) / wt, kb = (hi + wt - 1) / wt;
-          for (int64_t k = ka; k < kb && ok;) {
-            const int64_t u = k / line.tiles_p, ta = k - u * line.tiles_p, tb = min(line.tiles_p, ta + (kb - k));
-            const int64_t groups = seg == 0 ? S.row_tiles / 2 : 1;
-            const int64_t kvh = u / groups, rt = seg == 0 ? (u % groups) * 2 : S.row_tiles - 1;
-            const uint32_t* mk = a.w.mask_p + (kvh * S.row_tiles + rt) * p.Lp * 4;
-            ok = item(seg, kvh, rt * S.nb, (seg ? S.units[0] : 0) + u + blockIdx.x, p.ppages, 1, ptok, mk,
-                      seg == 0 ? mk + p.Lp * 4 : nullptr, 4, ta * ppt, min(pent, tb * ppt));
-            k += tb - ta;
+          more = done < total;  // a page is left over for another tile
+          if (lane == 0) {
+            td->flags = flags | first | (more ? 0 : F_LAST) | (cur == 0 ? F_EMPTY : 0);
+            td->n = cur;
+            td->vr = vr;
+            td->kvh = kvh;
+            td->b0 = b0;
+            td->slot = slot;
+            td->t0 = t0cur;
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[L::bDFull + d % L::kDescs]);
+          ++d;
+          first = 0;
         }
-        base += line.len[seg];
-      }
-      // own segment
-      if (active && ok && k1 > k0) {
-        int64_t b = s_start[0], c = s_start[1], k = k0;
-        while (k < k1 && b < p.B && ok) {
-          const int64_t tokens = own_tokens(p, b), ent = (tokens + p.page - 1) / p.page * sub;
-          const int64_t t = (ent + ppt - 1) / ppt;
-          while (k < k1 && k < (c + t) * p.Hkv && ok) {
-            const int64_t g = (k - c * p.Hkv) / t, ta = k - c * p.Hkv - g * t, tb = min(t, ta + (k1 - k));
-            ok = item(2, g, b, b * p.Hkv + g + blockIdx.x, p.bt + b * p.bts[0], p.bts[1], tokens,
-                      a.w.mask_o + (b * p.Hkv + g) * p.L * a.w.WO, nullptr, a.w.WO, ta * ppt, min(ent, tb * ppt));
-            k += tb - ta;
-          }
-          c += t;
-          ++b;
-        }
-      }
-      if (ok && acquire()) {
-        if (lane == 0) {
-          descs[d % L::kDescs].flags = F_END;
-          mbar_arrive(&bars[L::bDFull + d % L::kDescs]);
-        }
+        if (flags & F_END) break;
       }
     } else if (warp == kProducerWarp) {
       // ---------------------------------------------------------------- TMA producer
-      if (lane == 0) {
-        const int dc = (int)((p.D + 63) / 64);  // 64-column chunks
-        const int bn = S.bn;
-        uint32_t d = 0, seq = 0, nq = 0;
-        while (true) {
-          const uint32_t ds = d % L::kDescs;
-          if (!mbar_wait(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
-          const TileDesc& td = descs[ds];
-          const int flags = td.flags;
-          if (flags & F_END) break;
-          if (!(flags & F_EMPTY)) {
-            bool ok = true;
-            if (flags & F_FIRST) {
-              const int tiles = flags & F_PAIR ? 2 : 1;
-              for (int i = 0; i < tiles && ok; ++i, ++nq) {
-                const uint32_t qb = nq & 1;
-                if (!(ok = mbar_wait(&bars[L::bQEmpty + qb], ((nq >> 1) & 1) ^ 1, st))) break;
+      const int dc = (S.D + 63) / 64;  // 64-column chunks
+      const int bn = S.bn;
+      uint32_t d = 0, seq = 0, nq = 0;
+      bool ok = true;
+      while (ok) {
+        const uint32_t ds = d % L::kDescs;
+        if (!mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+        const TileDesc& td = descs[ds];
+        const int flags = td.flags;
+        if (flags & F_END) break;
+        if (!(flags & F_EMPTY)) {
+          const int kvh = td.kvh, b0 = td.b0, n = td.n, t0 = td.t0;
+          if (flags & F_FIRST) {
+            const int tiles = flags & F_PAIR ? 2 : 1;
+            for (int i = 0; i < tiles && ok; ++i, ++nq) {
+              const uint32_t qb = nq & 1;
+              if (!(ok = mbar_wait_warp(&bars[L::bQEmpty + qb], ((nq >> 1) & 1) ^ 1, st))) break;
+              if (elect_one()) {
                 unsigned char* dst = sm + L::kQ + qb * L::kTile;
-                const uint32_t rows = (uint32_t)((flags & F_OWN) ? p.G : S.nb * p.G);
+                const uint32_t rows = (uint32_t)((flags & F_OWN) ? S.G : S.nb * S.G);
                 mbar_arrive_expect_tx(&bars[L::bQFull + qb], rows * 128 * dc);
                 for (int c = 0; c < dc; ++c)
                   tma_load_4d(dst + c * (kT * 128), (flags & F_OWN) ? &a.tm_q1 : &a.tm_q, &bars[L::bQFull + qb], c * 64,
-                              0, td.kvh, td.b0 + i * S.nb);
+                              0, kvh, b0 + i * S.nb);
+              }
+              __syncwarp();
+            }
+          }
+          for (int kv = 0; kv < 2 && ok; ++kv, ++seq) {
+            const uint32_t sl = seq % L::kSlots;
+            if (!(ok = mbar_wait_warp(&bars[L::bEmpty + sl], ((seq / L::kSlots) & 1) ^ 1, st))) break;
+            if (elect_one()) {
+              unsigned char* dst = sm + L::kRing + sl * L::kTile;
+              mbar_arrive_expect_tx(&bars[L::bFull + sl], (uint32_t)(n * bn * 128 * dc));
+#pragma unroll 1
+              for (int j = 0; j < n; ++j, dst += bn * 128) {
+                const int phys = td.phys[j];
+                for (int c = 0; c < dc; ++c)
+                  tma_load_4d(dst + c * (kT * 128), kv ? &a.tm_v : &a.tm_k, &bars[L::bFull + sl], c * 64, t0, kvh, phys);
               }
             }
-            for (int kv = 0; kv < 2 && ok; ++kv, ++seq) {
-              const uint32_t sl = seq % L::kSlots;
-              if (!(ok = mbar_wait(&bars[L::bEmpty + sl], ((seq / L::kSlots) & 1) ^ 1, st))) break;
-              unsigned char* dst = sm + L::kRing + sl * L::kTile;
-              mbar_arrive_expect_tx(&bars[L::bFull + sl], (uint32_t)(td.n * bn * 128 * dc));
-              for (int j = 0; j < td.n; ++j)
-                for (int c = 0; c < dc; ++c)
-                  tma_load_4d(dst + c * (kT * 128) + j * bn * 128, kv ? &a.tm_v : &a.tm_k, &bars[L::bFull + sl], c * 64,
-                              td.t0, td.kvh, td.phys[j]);
-            }
-            if (!ok) break;
+            __syncwarp();
           }
-          mbar_arrive(&bars[L::bDEmpty + ds]);
-          ++d;
         }
+        if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
+        ++d;
       }
     } else if (warp == kMmaWarp) {
       // ---------------------------------------------------------------- MMA issuer
-      const int dk = (int)((p.D + 15) / 16);  // K steps of Q K^T, and N / 16 of P V
+      const int dk = (S.D + 15) / 16;  // K steps of Q K^T, and N / 16 of P V
       const uint32_t id_pv = idesc_f16(kT, dk * 16, BF16, false, true);
       struct Job {
         uint32_t tile;  // key tile index: K in ring entry 2 tile, V in 2 tile + 1
-        int lane, vr;
-        bool first, last, fix, rel;
+        int vr;
+        uint32_t bits;  // lane | J_*
       };
+      enum : uint32_t { J_FIRST = 2, J_LAST = 4, J_FIX = 8, J_REL = 16 };
       Job j0{}, j1{};  // pending P V products, j0 the older
       int np = 0;
-      uint32_t d = 0, tile = 0, job = 0, nq = 0, pc0 = 0, pc1 = 0, of0 = 0, of1 = 0;
-      int in_item = 0;  // key tiles of the item so far
-      bool ok = true;
-      auto pv = [&](const Job& j) -> bool {
-        const int g = j.lane;
-        const uint32_t seq = 2 * j.tile + 1, sl = seq % L::kSlots;
-        if (j.first) {  // O[g] has been read by the last item's epilogue
-          if (!mbar_wait_warp(&bars[L::bOFree + g], ((g ? of1 : of0) & 1) ^ 1, st)) return false;
-          if (g) ++of1; else ++of0;
-        }
-        if (!mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) return false;
-        unsigned char* vt = sm + L::kRing + sl * L::kTile;
-        const int n16 = (j.vr + 15) & ~15;
-        if (j.fix && (j.vr & 15)) {
-          // V rows past the valid keys meet P = 0: they must be finite, so they are cleared
-          const int rows = n16 - j.vr, units = rows * (DT / 8);
-          for (int i = lane; i < units; i += 32) {
-            const int rr = j.vr + i / (DT / 8), c = i % (DT / 8);
-            *reinterpret_cast<uint4*>(vt + (c >> 3) * (kT * 128) + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+      uint32_t d = 0, tile = 0, job = 0, nq = 0, pc[2] = {0, 0}, of[2] = {0, 0};
+      int in_item = 0;          // key tiles of the item so far
+      int left = 0, rts = 0;    // row tiles of the current key tile still to multiply, of how many
+      int flags = 0, vr = 0;
+      bool flush = false;
+      // One product per turn, P V of the older pending job as soon as two are pending (its P is
+      // then due first), else Q K^T of the next.
+      while (true) {
+        if (np == 2 || (flush && np > 0)) {
+          // ---- O[g] += P V
+          const uint32_t g = j0.bits & 1u;
+          const uint32_t seq = 2 * j0.tile + 1, sl = seq % L::kSlots;
+          if (j0.bits & J_FIRST) {  // O[g] has been read by the last item's epilogue
+            if (!mbar_wait_warp(&bars[L::bOFree + g], ((g ? of[1] : of[0]) & 1) ^ 1, st)) break;
+            if (g) ++of[1]; else ++of[0];
           }
-          fence_proxy_async_smem();
+          if (!mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
+          unsigned char* vt = sm + L::kRing + sl * L::kTile;
+          const int n16 = (j0.vr + 15) & ~15;
+          if ((j0.bits & J_FIX) && n16 != j0.vr) {
+            // V rows past the valid keys meet P = 0: they must be finite, so they are cleared
+            const int units = (n16 - j0.vr) * (DT / 8);
+#pragma unroll 1
+            for (int i = lane; i < units; i += 32) {
+              const int rr = j0.vr + i / (DT / 8), c = i % (DT / 8);
+              *reinterpret_cast<uint4*>(vt + (c >> 3) * (kT * 128) + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (!mbar_wait_warp(&bars[L::bPFull + g], (g ? pc[1] : pc[0]) & 1, st)) break;
+          if (g) ++pc[1]; else ++pc[0];
+          if (elect_one()) {
+            tc_fence_after();
+            const uint64_t vd = smem_desc(smem_u32(vt), kT * 128, 1024);
+            const uint32_t d_o = tmem + kColO + g * kT, a_p = tmem + kColS + g * kT;
+            const uint32_t acc = (j0.bits & J_FIRST) ? 0u : 1u;
+#pragma unroll
+            for (int kk = 0; kk < kT / 16; ++kk)
+              if (kk * 16 < n16)
+                tc_mma_f16_ts(d_o, a_p + kk * 8, desc_add(vd, kk * 16 * 128), id_pv, kk > 0 ? 1u : acc);
+            if (j0.bits & J_REL) tc_commit(&bars[L::bEmpty + sl]);
+            if (j0.bits & J_LAST) tc_commit(&bars[L::bODone + g]);
+          }
           __syncwarp();
-        }
-        if (!mbar_wait_warp(&bars[L::bPFull + g], (g ? pc1 : pc0) & 1, st)) return false;
-        if (g) ++pc1; else ++pc0;
-        if (lane == 0) {
-          tc_fence_after();
-          const uint64_t vd = smem_desc(smem_u32(vt), kT * 128, 1024);
-          const uint32_t d_o = tmem + kColO + g * kT, a_p = tmem + kColS + g * kT;
-          for (int kk = 0; kk < n16 / 16; ++kk)
-            tc_mma_f16_ts(d_o, a_p + kk * 8, desc_add(vd, kk * 16 * 128), id_pv, (!j.first || kk > 0) ? 1u : 0u);
-          if (j.rel) tc_commit(&bars[L::bEmpty + sl]);
-          if (j.last) tc_commit(&bars[L::bODone + g]);
-        }
-        __syncwarp();
-        return true;
-      };
-      while (ok) {
-        const uint32_t ds = d % L::kDescs;
-        if (np == 2) {
-          if (!(ok = pv(j0))) break;
           j0 = j1;
-          np = 1;
-        }
-        if (!(ok = mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st))) break;
-        const int flags = descs[ds].flags, vr = descs[ds].vr;
-        __syncwarp();
-        if (flags & F_END) break;
-        if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
-        ++d;
-        if (flags & F_EMPTY) {
-          // nothing to multiply: finish what is pending, so that the softmax groups, which wait for
-          // their last item's accumulators, go on releasing descriptors
-          if (np > 0) ok = pv(j0);
-          if (ok && np > 1) ok = pv(j1);
-          np = 0;
+          --np;
           continue;
         }
-        const int rts = flags & F_PAIR ? 2 : 1;
-        if (flags & F_FIRST) {
-          in_item = 0;
-          for (int i = 0; i < rts && ok; ++i)
-            ok = mbar_wait_warp(&bars[L::bQFull + ((nq + i) & 1)], ((nq + i) >> 1) & 1, st);
+        if (flush) {
+          if (flags & F_END) break;
+          flush = false;
         }
-        const uint32_t seq = 2 * tile, sl = seq % L::kSlots;
-        ok = ok && mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st);
-        if (!ok) break;
-        const int n16 = (vr + 15) & ~15;
-        const uint32_t id_qk = idesc_f16(kT, n16, BF16, false, false);
-        for (int i = 0; i < rts; ++i, ++job) {
-          const int g = job & 1;
-          if (np == 2) {
-            if (!(ok = pv(j0))) break;
-            j0 = j1;
-            np = 1;
-          }
-          if (lane == 0) {
-            tc_fence_after();
-            const uint64_t qd = smem_desc(smem_u32(sm + L::kQ + ((nq + i) & 1) * L::kTile), 16, 1024);
-            const uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
-            const uint32_t d_s = tmem + kColS + g * kT;
-            for (int kk = 0; kk < dk; ++kk) {
-              const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
-              tc_mma_f16(d_s, desc_add(qd, off), desc_add(kd, off), id_qk, kk > 0 ? 1u : 0u);
-            }
-            tc_commit(&bars[L::bSFull + g]);
-            if (i == rts - 1) tc_commit(&bars[L::bEmpty + sl]);
-            if (flags & F_LAST) tc_commit(&bars[L::bQEmpty + ((nq + i) & 1)]);
-          }
+        if (left == 0) {
+          // ---- the next key tile
+          const uint32_t ds = d % L::kDescs;
+          if (!mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+          flags = descs[ds].flags;
+          vr = descs[ds].vr;
           __syncwarp();
-          Job j;
-          j.tile = tile;
-          j.lane = g;
-          j.vr = vr;
-          j.fix = i == 0;
-          j.rel = i == rts - 1;
-          // the lane's first product of the item: its first tile's, or, where the lanes take the
-          // tiles in turn, its second tile's
-          j.first = in_item == 0 || (rts == 1 && in_item == 1);
-          j.last = (flags & F_LAST) != 0;
-          if (rts == 1 && j.last && in_item > 0) j0.last = true;  // the other lane's last, still pending
-          if (np == 0) j0 = j; else j1 = j;
-          ++np;
+          // at the end, and where an item has nothing to multiply, finish what is pending: the softmax
+          // groups wait for their last item's accumulators before they release more descriptors
+          flush = flags & (F_END | F_EMPTY);
+          if (lane == 0 && !(flags & F_END)) mbar_arrive(&bars[L::bDEmpty + ds]);
+          ++d;
+          if (flush) continue;
+          rts = left = flags & F_PAIR ? 2 : 1;
+          if (flags & F_FIRST) {
+            in_item = 0;
+            if (!mbar_wait_warp(&bars[L::bQFull + (nq & 1)], (nq >> 1) & 1, st)) break;
+            if (rts == 2 && !mbar_wait_warp(&bars[L::bQFull + ((nq + 1) & 1)], ((nq + 1) >> 1) & 1, st)) break;
+          }
+          if (!mbar_wait_warp(&bars[L::bFull + (2 * tile) % L::kSlots], ((2 * tile) / L::kSlots) & 1, st)) break;
         }
-        ++tile;
-        ++in_item;
-        if (flags & F_LAST) nq += rts;
+        // ---- S[g] = Q K^T
+        const uint32_t g = job & 1, sl = (2 * tile) % L::kSlots, qb = (nq + rts - left) & 1;
+        if (elect_one()) {
+          tc_fence_after();
+          const uint32_t id_qk = idesc_f16(kT, (vr + 15) & ~15, BF16, false, false);
+          const uint64_t qd = smem_desc(smem_u32(sm + L::kQ + qb * L::kTile), 16, 1024);
+          const uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
+          const uint32_t d_s = tmem + kColS + g * kT;
+#pragma unroll
+          for (int kk = 0; kk < DT / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
+            if (kk < dk) tc_mma_f16(d_s, desc_add(qd, off), desc_add(kd, off), id_qk, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(&bars[L::bSFull + g]);
+          if (left == 1) tc_commit(&bars[L::bEmpty + sl]);
+          if (flags & F_LAST) tc_commit(&bars[L::bQEmpty + qb]);
+        }
+        __syncwarp();
+        // the lane's first product of the item: its first tile's, or, where the lanes take the tiles in
+        // turn, its second tile's
+        Job j;
+        j.tile = tile;
+        j.vr = vr;
+        j.bits = g | ((in_item == 0 || (rts == 1 && in_item == 1)) ? J_FIRST : 0u) | ((flags & F_LAST) ? J_LAST : 0u) |
+                 (left == rts ? J_FIX : 0u) | (left == 1 ? J_REL : 0u);
+        if (rts == 1 && (flags & F_LAST) && in_item > 0) j0.bits |= J_LAST;  // the other lane's last, still pending
+        if (np == 0) j0 = j; else j1 = j;
+        ++np;
+        ++job;
+        if (--left == 0) {
+          ++tile;
+          ++in_item;
+          if (flags & F_LAST) nq += rts;
+        }
       }
-      if (ok && np > 0) ok = pv(j0);
-      if (ok && np > 1) pv(j1);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -702,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t col_s = kColS + grp * kT, col_o = kColO + grp * kT;
     const float sc2 = a.scale2;
-    const int G = (int)p.G, D4 = (int)p.D / 4;
+    const int G = S.G, D4 = S.D / 4;
     uint32_t d = 0, job = 0, sc = 0, od = 0;
     float m_used = -INFINITY, l_sum = 0.f;
     bool had = false;
@@ -720,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         m_used = -INFINITY;
         l_sum = 0.f;
         had = false;
-        row_ok = own ? rl < G : rl < S.nb * G && (int64_t)td.b0 + (pair ? sub * S.nb : 0) + rl / G < p.B;
+        row_ok = own ? rl < G : rl < S.nb * G && td.b0 + (pair ? sub * S.nb : 0) + rl / G < S.B;
       }
       const bool mine = !empty && (pair || (int)(job & 1) == grp);
       // keys in groups of 8 that this row attends (pages are multiples of 8 rows)
@@ -741,62 +790,81 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         ++sc;
         tc_fence_after();
         if (__any_sync(0xffffffffu, row_ok)) {
-          const int n16 = (vr + 15) & ~15;
-          float s[kT];
+          const int nch = (vr + 31) >> 5;  // 32-key chunks with valid keys
+          if (vr & 31) {
+            // the last chunk's columns past the valid keys hold whatever was there: -inf in place
+            float x[32];
+            tmem_ld32(lane_addr + col_s + (nch - 1) * 32, x);
+            tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < kT / 32; ++c) {
-            float chunk[32];
-            if (c * 32 < n16) {
-              tmem_ld32(lane_addr + col_s + c * 32, chunk);
+            for (int i = 0; i < 32; ++i) x[i] = i < (vr & 31) ? x[i] : -INFINITY;
+            tmem_st32(lane_addr + col_s + (nch - 1) * 32, x);
+            tmem_wait_st();
+          }
+          // Row maximum, per group of 8 keys so that a masked group falls away by selection.
+          float mraw = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < nch; c += 2) {
+            float x[64];
+            tmem_ld32(lane_addr + col_s + c * 32, reinterpret_cast<float(&)[32]>(x[0]));
+            if (c + 1 < nch) tmem_ld32(lane_addr + col_s + c * 32 + 32, reinterpret_cast<float(&)[32]>(x[32]));
+            tmem_wait_ld();
+            const int nk = c + 1 < nch ? 8 : 4;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[c * 32 + i] = chunk[i];
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) s[c * 32 + i] = -INFINITY;
+            for (int k = 0; k < 8; ++k) {
+              const float* y = x + 8 * k;
+              const float mg = fmax3(fmax3(y[0], y[1], y[2]), fmax3(y[3], y[4], y[5]), fmaxf(y[6], y[7]));
+              if (k < nk) mraw = fmaxf(mraw, (gm >> (c * 4 + k)) & 1u ? mg : -INFINITY);
             }
           }
-          tmem_wait_ld();
-          // masked keys by selection (-inf), so that nothing they hold matters
-          if (__any_sync(0xffffffffu, gm != 0xffffu)) {
-#pragma unroll
-            for (int c = 0; c < kT; ++c) s[c] = (gm >> (c >> 3)) & 1u ? s[c] : -INFINITY;
-          }
-          if (vr < kT) {
-#pragma unroll
-            for (int c = 0; c < kT; ++c) s[c] = c < vr ? s[c] : -INFINITY;
-          }
-          float mx[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) mx[i] = fmaxf(s[2 * i], s[2 * i + 1]);
-#pragma unroll
-          for (int c = 16; c < kT; c += 2) mx[(c >> 1) & 7] = fmax3(mx[(c >> 1) & 7], s[c], s[c + 1]);
-          const float mraw = fmaxf(fmax3(mx[0], mx[1], mx[2]), fmax3(fmax3(mx[3], mx[4], mx[5]), mx[6], mx[7]));
           const float mt = mraw * sc2;
           float m_new = m_used;
           if (mt > -INFINITY && (m_used == -INFINITY || mt > m_used + kRescaleThreshold)) m_new = mt;
           const float m_ref = m_new == -INFINITY ? 0.f : m_new;
           const float alpha = m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_ref);
           const bool rescale = m_new != m_used && m_used != -INFINITY;
-          const uint64_t scale_x2 = f32x2(sc2, sc2), bias_x2 = f32x2(-m_ref, -m_ref);
-          uint64_t rs[4] = {0, 0, 0, 0};
+          const uint64_t scale_x2 = f32x2(sc2, sc2);
+          uint64_t rs0 = 0, rs1 = 0;
+          // Exponentials and P, 32 keys at a time from a second read of S: a loop this short stays in
+          // the instruction cache beside the MMA warp's code, which the 128 unrolled columns of a
+          // single read evict.  A masked group's bias is -inf.
+          float xa[32], xb[32];
+          auto chunk = [&](const float(&x)[32], int c) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int c = 0; c < kT / 32; ++c) {
-            if (c * 32 < n16) {
-              uint32_t pk[16];
+            for (int k = 0; k < 4; ++k) {
+              const float bk = (gm >> (c * 4 + k)) & 1u ? -m_ref : -INFINITY;
+              const uint64_t bias_x2 = f32x2(bk, bk);
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
+              for (int i = k * 8; i < k * 8 + 8; i += 2) {
                 float e0, e1;
-                f32x2_split(fma_f32x2(f32x2(s[c * 32 + i], s[c * 32 + i + 1]), scale_x2, bias_x2), e0, e1);
+                f32x2_split(fma_f32x2(f32x2(x[i], x[i + 1]), scale_x2, bias_x2), e0, e1);
                 const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
-                rs[(i >> 1) & 3] = add_f32x2(rs[(i >> 1) & 3], f32x2(p0, p1));
+                if (i & 2) rs1 = add_f32x2(rs1, f32x2(p0, p1));
+                else rs0 = add_f32x2(rs0, f32x2(p0, p1));
                 pk[i / 2] = pack2(p0, p1, BF16);
               }
-              tmem_st16(lane_addr + col_s + c * 16, pk);
+            }
+            tmem_st16(lane_addr + col_s + c * 16, pk);
+          };
+          tmem_ld32(lane_addr + col_s, xa);
+          tmem_wait_ld();
+#pragma unroll 1
+          for (int c = 0; c < nch; c += 2) {
+            const bool two = c + 1 < nch;
+            if (two) tmem_ld32(lane_addr + col_s + c * 32 + 32, xb);
+            chunk(xa, c);
+            if (two) {
+              tmem_wait_ld();
+              if (c + 2 < nch) tmem_ld32(lane_addr + col_s + c * 32 + 64, xa);
+              chunk(xb, c + 1);
+              tmem_wait_ld();
             }
           }
           // S(i) being complete implies that the lane's last P V is: O[g] may be rescaled here
           if (had && __any_sync(0xffffffffu, rescale)) {
             const float f = rescale ? alpha : 1.f;
+#pragma unroll 1
             for (int c = 0; c < DT / 32; ++c) {
               float o[32];
               tmem_ld32(lane_addr + col_o + c * 32, o);
@@ -808,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           }
           tmem_wait_st();
           float r0, r1;
-          f32x2_split(add_f32x2(add_f32x2(rs[0], rs[1]), add_f32x2(rs[2], rs[3])), r0, r1);
+          f32x2_split(add_f32x2(rs0, rs1), r0, r1);
           l_sum = (m_used == -INFINITY ? 0.f : l_sum * alpha) + (r0 + r1);
           m_used = m_new;
         }
@@ -818,8 +886,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       }
       if (!(flags & F_LAST)) continue;
       // ---------------------------------------------------------------- the item's partial state
-      const int64_t state = (int64_t)slot * 2 + sub;
       const int rows = own ? G : kT;
+      const int64_t state = (int64_t)slot * 2 + sub;
       float2* ml = (own ? a.w.ml_o : a.w.ml_p) + state * rows;
       float4* acc = (own ? a.w.acc_o : a.w.acc_p) + state * D4 * rows;
       if (row_ok) ml[rl] = make_float2(had ? m_used : -INFINITY, l_sum);
@@ -828,19 +896,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         ++od;
         tc_fence_after();
         if (__any_sync(0xffffffffu, row_ok)) {
+          const bool put = row_ok && (m_used != -INFINITY || l_sum != 0.f);
+          float4* dst = acc + rl;
+#pragma unroll 1
+          for (int c = 0; c * 8 < D4; ++c, dst += 8 * rows) {
+            float o[32];
+            tmem_ld32(lane_addr + col_o + c * 32, o);
+            tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < DT / 32; ++c) {
-            if (c * 8 < D4) {
-              float o[32];
-              tmem_ld32(lane_addr + col_o + c * 32, o);
-              tmem_wait_ld();
-              if (row_ok && (m_used != -INFINITY || l_sum != 0.f)) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  if (c * 8 + i < D4)
-                    acc[(int64_t)(c * 8 + i) * rows + rl] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-              }
-            }
+            for (int i = 0; i < 8; ++i)
+              if (put && c * 8 + i < D4) dst[i * rows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
         tc_fence_before();
@@ -868,7 +933,7 @@ constexpr int kCombThreads = 256;
 // such rows are computed again over their attended keys alone.  Costs tokens x ~100 cycles: only
 // non-finite values get here.
 template <typename T>
-__device__ void exact_row(const PrefixParams& p, int64_t b, int64_t h, float scale2) {
+__device__ __noinline__ void exact_row(const PrefixParams& p, int64_t b, int64_t h, float scale2) {
   const int lane = threadIdx.x & 31;
   const int64_t g = h / p.G, ptok = prefix_tokens(p), otok = own_tokens(p, b);
   const int64_t pp = (ptok + p.page - 1) / p.page, n = pp + (otok + p.page - 1) / p.page;
@@ -911,32 +976,29 @@ __global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const Pref
   __shared__ float4 s_acc[kCombThreads];
   __shared__ float2 s_ml[kCombThreads];
   __shared__ unsigned s_bad[4];  // rows (of the group) to compute again
-  const int64_t b = blockIdx.x / p.Hkv, g = blockIdx.x % p.Hkv;
-  const int G = (int)p.G, D4 = (int)p.D / 4, tid = threadIdx.x;
+  const int G = s.G, D4 = s.D / 4, tid = threadIdx.x;
+  const int b = blockIdx.x / s.Hkv, g = blockIdx.x - b * s.Hkv;
   if (tid < 4) s_bad[tid] = 0;
   pdl_wait();
-  const Line line = make_line(p, s, w.cum[p.B]);
+  const int cum0 = w.cum[b], t_own = w.cum[b + 1] - cum0;
+  const Line line = make_line(s, tokens_in(p.plen_dev ? *p.plen_dev : (int)p.plen, s.Lp, s.page), w.cum[s.B]);
   // pieces of the prefix: row tile rt of KV head g, and of the request's own pages
-  const int rt = (int)(b / s.nb), r0 = (int)(b - (int64_t)rt * s.nb) * G;
-  int64_t sp0 = 0, so0 = 0;  // first slots
-  int npre = 0, nown = 0, sub0 = 0, subs = 1;
-  if (line.W > 0 && line.tiles_p > 0) {
-    const int pairs = s.row_tiles / 2;
-    const bool pair = rt < 2 * pairs;
-    const int64_t u = pair ? g * pairs + rt / 2 : s.units[0] + g;
-    const int64_t x = pair ? u * line.tiles_p * kWPair : line.len[0] + g * line.tiles_p * kWOne;
-    const int64_t i0 = range_of(line, x), i1 = range_of(line, x + (line.tiles_p - 1) * (pair ? kWPair : kWOne));
+  const int rt = b / s.nb, r0 = (b - rt * s.nb) * G, pairs = s.row_tiles / 2;
+  const bool pair = rt < 2 * pairs;
+  const int wt = pair ? kWPair : kWOne, subs = pair ? 1 : 2, sub0 = pair ? rt & 1 : 0;
+  const int u = pair ? g * pairs + rt / 2 : s.units[0] + g;
+  int sp0 = 0, so0 = 0, npre = 0, nown = 0;  // first slots, pieces
+  if (line.tiles_p > 0) {
+    const int64_t x = pair ? (int64_t)u * line.tiles_p * kWPair : line.len[0] + (int64_t)g * line.tiles_p * kWOne;
+    const int i0 = range_of(line, x);
     sp0 = u + i0;
-    npre = (int)(i1 - i0 + 1);
-    sub0 = pair ? rt & 1 : 0;
-    subs = pair ? 1 : 2;
+    npre = range_of(line, x + (int64_t)(line.tiles_p - 1) * wt) - i0 + 1;
   }
-  const int t_own = w.cum[b + 1] - w.cum[b];
   if (t_own > 0) {
-    const int64_t x = line.len[0] + line.len[1] + ((int64_t)w.cum[b] * p.Hkv + g * t_own) * kWOne;
-    const int64_t i0 = range_of(line, x), i1 = range_of(line, x + (int64_t)(t_own - 1) * kWOne);
-    so0 = b * p.Hkv + g + i0;
-    nown = (int)(i1 - i0 + 1);
+    const int64_t x = line.len[0] + line.len[1] + ((int64_t)cum0 * s.Hkv + g * t_own) * kWOne;
+    const int i0 = range_of(line, x);
+    so0 = b * s.Hkv + g + i0;
+    nown = range_of(line, x + (int64_t)(t_own - 1) * kWOne) - i0 + 1;
   }
   const int total = npre * subs + nown * 2;
   const int cells = G * D4;                    // float4 outputs of the group
@@ -960,11 +1022,11 @@ __global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const Pref
         x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (k < total) {
           if (k < npre * subs) {
-            const int64_t state = (sp0 + k / subs) * 2 + sub0 + k % subs;
+            const int64_t state = subs == 2 ? sp0 * 2 + k : (sp0 + k) * 2 + sub0;
             ml[u] = __ldcg(w.ml_p + state * kT + r0 + hh);
             x[u] = __ldcg(w.acc_p + (state * D4 + c4) * kT + r0 + hh);
           } else {
-            const int64_t state = so0 * 2 + (k - npre * subs);
+            const int64_t state = (int64_t)so0 * 2 + (k - npre * subs);
             ml[u] = __ldcg(w.ml_o + state * G + hh);
             x[u] = __ldcg(w.acc_o + (state * D4 + c4) * G + hh);
           }
@@ -1005,12 +1067,12 @@ __global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const Pref
       // an infinite weight or a NaN anywhere makes this sum NaN or infinite
       if (!(fabsf(acc.x) + fabsf(acc.y) + fabsf(acc.z) + fabsf(acc.w) + fabsf(Ls) < INFINITY))
         atomicOr(&s_bad[hh >> 5], 1u << (hh & 31));
-      T* o = static_cast<T*>(p.out) + b * p.os[0] + (g * G + hh) * p.os[1] + 4 * c4;
+      T* o = static_cast<T*>(p.out) + b * p.os[0] + (int64_t)(g * G + hh) * p.os[1] + 4 * c4;
       o[0] = from_f32<T>(acc.x * inv);
       o[1] = from_f32<T>(acc.y * inv);
       o[2] = from_f32<T>(acc.z * inv);
       o[3] = from_f32<T>(acc.w * inv);
-      if (p.lse && c4 == 0) p.lse[b * p.H + g * G + hh] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
+      if (p.lse && c4 == 0) p.lse[(int64_t)b * s.Hkv * G + g * G + hh] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
     }
   }
   __syncthreads();
@@ -1042,16 +1104,21 @@ int launch_main(const Args& a, bool dependent, cudaStream_t stream) {
 
 bool prefix_fast_shape(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page) {
   return (dtype == SA_BF16 || dtype == SA_F16) && D % 8 == 0 && D <= 128 && page % 8 == 0 && H / Hkv <= kT &&
-         H <= 32 * kMaxHeadWords && B * Hkv <= INT32_MAX / 2;
+         H <= 32 * kMaxHeadWords && B * Hkv <= (1 << 26) && page <= (1 << 20);
 }
 
 int64_t prefix_fast_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page, int64_t Lp, int64_t L) {
-  return (int64_t)carve(nullptr, B, Hkv, H / Hkv, D, Lp, L, make_split(B, H / Hkv, Hkv, page), nullptr);
+  return (int64_t)carve(nullptr, make_split(B, H / Hkv, Hkv, page, Lp, L, D), nullptr);
 }
 
 bool prefix_fast_eligible(const PrefixParams& p, int dtype) {
   if (!prefix_fast_shape(dtype, p.B, p.H, p.Hkv, p.D, p.page)) return false;
   if (p.num_pages < 1 || p.num_pages > INT32_MAX) return false;
+  // weighted key tiles of the whole batch stay below 2^31
+  const int64_t span = std::max<int64_t>(8, std::min<int64_t>(p.page, kT));
+  if ((double)p.B * p.Hkv * (p.L + 1) * (p.page / span + 1) * kWPair > 1e9 ||
+      (double)p.B * p.Hkv * (p.Lp + 1) * (p.page / span + 1) * kWPair > 1e9)
+    return false;
   if (reinterpret_cast<uintptr_t>(p.q) % 16 || reinterpret_cast<uintptr_t>(p.kc) % 16 ||
       reinterpret_cast<uintptr_t>(p.vc) % 16)
     return false;
@@ -1064,9 +1131,17 @@ bool prefix_fast_eligible(const PrefixParams& p, int dtype) {
 
 int launch_prefix_fast(const PrefixParams& p, int dtype, void* workspace, cudaStream_t stream) {
   Args a{};
-  a.p = p;
-  a.s = make_split(p.B, p.G, p.Hkv, p.page);
-  carve(workspace, p.B, p.Hkv, p.G, p.D, p.Lp, p.L, a.s, &a.w);
+  a.s = make_split(p.B, p.G, p.Hkv, p.page, p.Lp, p.L, p.D);
+  carve(workspace, a.s, &a.w);
+  a.ppages = p.ppages;
+  a.bt = p.bt;
+  a.bts0 = p.bts[0];
+  a.bts1 = p.bts[1];
+  a.ctx = p.ctx;
+  a.plen_dev = p.plen_dev;
+  a.plen = (int)p.plen;
+  a.num_pages = (int)p.num_pages;
+  a.status = p.status;
   a.scale2 = (1.0f / sqrtf((float)p.D)) * kLog2e;
   a.masked = p.r > 0;
   // query rows as (D, G, KV head, request): a box of nb requests is one row tile

@@ -103,8 +103,15 @@ struct Split {
   int B, G, Hkv, page, Lp, L, D;
 };
 
+// The partial states of one (request, KV head): n states from `first`, `stride` apart.
+struct Pieces {
+  int first_p, n_p, stride_p, r0;  // prefix: r0 = the request's first row in the row tile
+  int first_o, n_o, pad[2];        // own, one apart
+};
+static_assert(sizeof(Pieces) == 32, "Pieces");
+
 struct Ws {
-  int* cum;           // [B + 1] own tiles of requests before b (one KV head)
+  Pieces* plan;       // [B][Hkv] where a request's partial states are
   uint32_t* mask_p;   // [Hkv][row_tiles][Lp][4]
   uint32_t* mask_o;   // [B][Hkv][L][WO]
   float2* ml_p;       // [prefix slots][2][128]
@@ -164,7 +171,7 @@ size_t carve(void* base, const Split& s, Ws* w) {
   Ws t;
   t.WO = G <= 32 ? 1 : 4;
   const size_t sp = (size_t)s.units[0] + s.units[1] + s.grid, so = (size_t)(B * Hkv + s.grid);
-  t.cum = reinterpret_cast<int*>(take((size_t)(B + 1) * 4));
+  t.plan = reinterpret_cast<Pieces*>(take((size_t)B * Hkv * sizeof(Pieces)));
   t.mask_p = reinterpret_cast<uint32_t*>(take((size_t)Hkv * s.row_tiles * Lp * 16));
   t.mask_o = reinterpret_cast<uint32_t*>(take((size_t)B * Hkv * L * t.WO * 4));
   t.ml_p = reinterpret_cast<float2*>(take(sp * 2 * kT * 8));
@@ -415,14 +422,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
 #pragma unroll 1
     for (int b = bfirst; b < bend; ++b) {
       const int t = tiles_of(S, tokens_in(a.ctx[b], S.L, S.page));
-      if (blockIdx.x == 0) a.w.cum[b] = c;
       if (k0 >= c * S.Hkv && k0 < (c + t) * S.Hkv) {
         s_start[0] = b;
         s_start[1] = c;
       }
       c += t;
     }
-    if (blockIdx.x == 0 && threadIdx.x == kThreads - 1) a.w.cum[S.B] = own_total;
   }
   __syncthreads();
   pdl_trigger();
@@ -622,7 +627,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         ++d;
       }
     } else if (warp == kMmaWarp) {
-      // ---------------------------------------------------------------- MMA issuer
+      // ---------------------------------------------------------------- MMA issuer (one thread)
+      if (elect_one()) {
       const int dk = (S.D + 15) / 16;  // K steps of Q K^T, and N / 16 of P V
       const uint32_t id_pv = idesc_f16(kT, dk * 16, BF16, false, true);
       struct Job {
@@ -630,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         int vr;
         uint32_t bits;  // lane | J_*
       };
-      enum : uint32_t { J_FIRST = 2, J_LAST = 4, J_FIX = 8, J_REL = 16 };
+      enum : uint32_t { J_FIRST = 2, J_LAST = 4, J_REL = 8 };
       Job j0{}, j1{};  // pending P V products, j0 the older
       int np = 0;
       uint32_t d = 0, tile = 0, job = 0, nq = 0, pc[2] = {0, 0}, of[2] = {0, 0};
@@ -646,28 +652,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           const uint32_t g = j0.bits & 1u;
           const uint32_t seq = 2 * j0.tile + 1, sl = seq % L::kSlots;
           if (j0.bits & J_FIRST) {  // O[g] has been read by the last item's epilogue
-            if (!mbar_wait_warp(&bars[L::bOFree + g], ((g ? of[1] : of[0]) & 1) ^ 1, st)) break;
+            if (!mbar_wait(&bars[L::bOFree + g], ((g ? of[1] : of[0]) & 1) ^ 1, st)) break;
             if (g) ++of[1]; else ++of[0];
           }
-          if (!mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
-          unsigned char* vt = sm + L::kRing + sl * L::kTile;
+          if (!mbar_wait(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
           const int n16 = (j0.vr + 15) & ~15;
-          if ((j0.bits & J_FIX) && n16 != j0.vr) {
-            // V rows past the valid keys meet P = 0: they must be finite, so they are cleared
-            const int units = (n16 - j0.vr) * (DT / 8);
-#pragma unroll 1
-            for (int i = lane; i < units; i += 32) {
-              const int rr = j0.vr + i / (DT / 8), c = i % (DT / 8);
-              *reinterpret_cast<uint4*>(vt + (c >> 3) * (kT * 128) + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-          if (!mbar_wait_warp(&bars[L::bPFull + g], (g ? pc[1] : pc[0]) & 1, st)) break;
+          if (!mbar_wait(&bars[L::bPFull + g], (g ? pc[1] : pc[0]) & 1, st)) break;
           if (g) ++pc[1]; else ++pc[0];
-          if (elect_one()) {
+          {
             tc_fence_after();
-            const uint64_t vd = smem_desc(smem_u32(vt), kT * 128, 1024);
+            const uint64_t vd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), kT * 128, 1024);
             const uint32_t d_o = tmem + kColO + g * kT, a_p = tmem + kColS + g * kT;
             const uint32_t acc = (j0.bits & J_FIRST) ? 0u : 1u;
 #pragma unroll
@@ -677,7 +671,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
             if (j0.bits & J_REL) tc_commit(&bars[L::bEmpty + sl]);
             if (j0.bits & J_LAST) tc_commit(&bars[L::bODone + g]);
           }
-          __syncwarp();
           j0 = j1;
           --np;
           continue;
@@ -689,27 +682,26 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         if (left == 0) {
           // ---- the next key tile
           const uint32_t ds = d % L::kDescs;
-          if (!mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+          if (!mbar_wait(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
           flags = descs[ds].flags;
           vr = descs[ds].vr;
-          __syncwarp();
           // at the end, and where an item has nothing to multiply, finish what is pending: the softmax
           // groups wait for their last item's accumulators before they release more descriptors
           flush = flags & (F_END | F_EMPTY);
-          if (lane == 0 && !(flags & F_END)) mbar_arrive(&bars[L::bDEmpty + ds]);
+          if (!(flags & F_END)) mbar_arrive(&bars[L::bDEmpty + ds]);
           ++d;
           if (flush) continue;
           rts = left = flags & F_PAIR ? 2 : 1;
           if (flags & F_FIRST) {
             in_item = 0;
-            if (!mbar_wait_warp(&bars[L::bQFull + (nq & 1)], (nq >> 1) & 1, st)) break;
-            if (rts == 2 && !mbar_wait_warp(&bars[L::bQFull + ((nq + 1) & 1)], ((nq + 1) >> 1) & 1, st)) break;
+            if (!mbar_wait(&bars[L::bQFull + (nq & 1)], (nq >> 1) & 1, st)) break;
+            if (rts == 2 && !mbar_wait(&bars[L::bQFull + ((nq + 1) & 1)], ((nq + 1) >> 1) & 1, st)) break;
           }
-          if (!mbar_wait_warp(&bars[L::bFull + (2 * tile) % L::kSlots], ((2 * tile) / L::kSlots) & 1, st)) break;
+          if (!mbar_wait(&bars[L::bFull + (2 * tile) % L::kSlots], ((2 * tile) / L::kSlots) & 1, st)) break;
         }
         // ---- S[g] = Q K^T
         const uint32_t g = job & 1, sl = (2 * tile) % L::kSlots, qb = (nq + rts - left) & 1;
-        if (elect_one()) {
+        {
           tc_fence_after();
           const uint32_t id_qk = idesc_f16(kT, (vr + 15) & ~15, BF16, false, false);
           const uint64_t qd = smem_desc(smem_u32(sm + L::kQ + qb * L::kTile), 16, 1024);
@@ -724,14 +716,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           if (left == 1) tc_commit(&bars[L::bEmpty + sl]);
           if (flags & F_LAST) tc_commit(&bars[L::bQEmpty + qb]);
         }
-        __syncwarp();
         // the lane's first product of the item: its first tile's, or, where the lanes take the tiles in
         // turn, its second tile's
         Job j;
         j.tile = tile;
         j.vr = vr;
         j.bits = g | ((in_item == 0 || (rts == 1 && in_item == 1)) ? J_FIRST : 0u) | ((flags & F_LAST) ? J_LAST : 0u) |
-                 (left == rts ? J_FIX : 0u) | (left == 1 ? J_REL : 0u);
+                 (left == 1 ? J_REL : 0u);
         if (rts == 1 && (flags & F_LAST) && in_item > 0) j0.bits |= J_LAST;  // the other lane's last, still pending
         if (np == 0) j0 = j; else j1 = j;
         ++np;
@@ -741,6 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           ++in_item;
           if (flags & F_LAST) nq += rts;
         }
+      }
       }
     }
   } else {
@@ -752,7 +744,47 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     const uint32_t col_s = kColS + grp * kT, col_o = kColO + grp * kT;
     const float sc2 = a.scale2;
     const int G = S.G, D4 = S.D / 4;
-    uint32_t d = 0, job = 0, sc = 0, od = 0;
+    if (warp == 4) {
+      // Before its first scores arrive, this warp writes down for the join where the partial states of
+      // the CTA's share of the requests are (lane = KV head): the CTAs whose ranges hold the first and
+      // last tile of the prefix unit and of the own unit.
+      const int per = (S.B + (int)gridDim.x - 1) / (int)gridDim.x;
+      const int ba = min(S.B, (int)blockIdx.x * per), bz = min(S.B, ba + per);
+      int cum = 0;
+      if (ba < bz) {
+#pragma unroll 4
+        for (int b = lane; b < ba; b += 32) cum += tiles_of(S, tokens_in(a.ctx[b], S.L, S.page));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) cum += __shfl_xor_sync(0xffffffffu, cum, o);
+      }
+#pragma unroll 1
+      for (int b = ba; b < bz; ++b) {
+        const int t = tiles_of(S, tokens_in(a.ctx[b], S.L, S.page));
+        const int rt = b / S.nb, pairs = S.row_tiles / 2;
+        const bool pr = rt < 2 * pairs;
+#pragma unroll 1
+        for (int g = lane; g < S.Hkv; g += 32) {
+          Pieces q{0, 0, pr ? 2 : 1, (b - rt * S.nb) * G, 0, 0, {0, 0}};
+          if (line.tiles_p > 0) {
+            const int u = pr ? g * pairs + rt / 2 : S.units[0] + g, wt = pr ? kWPair : kWOne;
+            const int64_t x = pr ? (int64_t)u * line.tiles_p * kWPair : line.len[0] + (int64_t)g * line.tiles_p * kWOne;
+            const int i0 = range_of(line, x);
+            q.n_p = (range_of(line, x + (int64_t)(line.tiles_p - 1) * wt) - i0 + 1) * (pr ? 1 : 2);
+            q.first_p = (u + i0) * 2 + (pr ? rt & 1 : 0);
+          }
+          if (t > 0) {
+            const int64_t x = own_base + ((int64_t)cum * S.Hkv + g * t) * kWOne;
+            const int i0 = range_of(line, x);
+            q.n_o = (range_of(line, x + (int64_t)(t - 1) * kWOne) - i0 + 1) * 2;
+            q.first_o = (b * S.Hkv + g + i0) * 2;
+          }
+          a.w.plan[(int64_t)b * S.Hkv + g] = q;
+        }
+        cum += t;
+      }
+      __syncwarp();
+    }
+    uint32_t d = 0, job = 0, tile = 0, sc = 0, od = 0;
     float m_used = -INFINITY, l_sum = 0.f;
     bool had = false;
     int sub = 0;        // which of the slot's two states this group writes
@@ -784,7 +816,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
       ++d;
-      if (!empty) job += pair ? 2 : 1;
+      if (!empty) {
+        job += pair ? 2 : 1;
+        ++tile;
+      }
       if (mine) {
         if (!mbar_wait_warp(&bars[L::bSFull + grp], sc & 1, st)) break;
         ++sc;
@@ -880,6 +915,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           l_sum = (m_used == -INFINITY ? 0.f : l_sum * alpha) + (r0 + r1);
           m_used = m_new;
         }
+        if (vr & 15) {
+          // V rows past the valid keys meet P = 0 in the product's last K step: they must be finite, so
+          // they are cleared (in a pair tile by both groups, with the same zeros)
+          const uint32_t seq = 2 * (tile - 1) + 1, sl = seq % L::kSlots;
+          if (!mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
+          unsigned char* vt = sm + L::kRing + sl * L::kTile;
+          const int units = (16 - (vr & 15)) * (DT / 8);
+#pragma unroll 1
+          for (int i = rl; i < units; i += kGroupThreads) {
+            const int rr = vr + i / (DT / 8), c = i % (DT / 8);
+            *reinterpret_cast<uint4*>(vt + (c >> 3) * (kT * 128) + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
         tc_fence_before();
         mbar_arrive(&bars[L::bPFull + grp]);
         had = true;
@@ -925,7 +974,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
 // ---------------------------------------------------------------------------------------
 // join of the partial states, one CTA per (request, KV head)
 // ---------------------------------------------------------------------------------------
-constexpr int kCombThreads = 256;
+constexpr int kCombThreads = 512;  // at most
 
 // Row (b, h) by itself, one warp: for rows whose joined state is not finite.  In the tensor-core
 // product a page's V meets every row of the tile, with weight 0 where the row does not attend
@@ -970,48 +1019,48 @@ __device__ __noinline__ void exact_row(const PrefixParams& p, int64_t b, int64_t
   if (p.lse && lane == 0) p.lse[b * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
+// Thread = (head, float4 of the output); blockDim / cells groups of threads share a unit's states
+// where there are many of them and few units, and are joined through shared memory.  A chain of
+// three dependent round trips (plan, states, store): bound by latency, so all of a group's loads of
+// a round are issued together and nothing is divided here.
 template <typename T>
-__global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const PrefixParams p, const Split s, const Ws w,
-                                                                      float scale2) {
+__global__ void __launch_bounds__(kCombThreads, 2) prefix_combine_kernel(const __grid_constant__ PrefixParams p,
+                                                                         const Split s, const Ws w,
+                                                                         float scale2) {
   __shared__ float4 s_acc[kCombThreads];
   __shared__ float2 s_ml[kCombThreads];
   __shared__ unsigned s_bad[4];  // rows (of the group) to compute again
   const int G = s.G, D4 = s.D / 4, tid = threadIdx.x;
   const int b = blockIdx.x / s.Hkv, g = blockIdx.x - b * s.Hkv;
+  const int cells = G * D4;                       // float4 outputs of the unit
+  const int cpb = min(cells, (int)blockDim.x);    // cells per pass
+  const int CG = (int)blockDim.x / cpb;           // thread groups over the states
+  const int cg = tid / cpb, ci = tid - cg * cpb;
   if (tid < 4) s_bad[tid] = 0;
   pdl_wait();
-  const int cum0 = w.cum[b], t_own = w.cum[b + 1] - cum0;
-  const Line line = make_line(s, tokens_in(p.plen_dev ? *p.plen_dev : (int)p.plen, s.Lp, s.page), w.cum[s.B]);
-  // pieces of the prefix: row tile rt of KV head g, and of the request's own pages
-  const int rt = b / s.nb, r0 = (b - rt * s.nb) * G, pairs = s.row_tiles / 2;
-  const bool pair = rt < 2 * pairs;
-  const int wt = pair ? kWPair : kWOne, subs = pair ? 1 : 2, sub0 = pair ? rt & 1 : 0;
-  const int u = pair ? g * pairs + rt / 2 : s.units[0] + g;
-  int sp0 = 0, so0 = 0, npre = 0, nown = 0;  // first slots, pieces
-  if (line.tiles_p > 0) {
-    const int64_t x = pair ? (int64_t)u * line.tiles_p * kWPair : line.len[0] + (int64_t)g * line.tiles_p * kWOne;
-    const int i0 = range_of(line, x);
-    sp0 = u + i0;
-    npre = range_of(line, x + (int64_t)(line.tiles_p - 1) * wt) - i0 + 1;
-  }
-  if (t_own > 0) {
-    const int64_t x = line.len[0] + line.len[1] + ((int64_t)cum0 * s.Hkv + g * t_own) * kWOne;
-    const int i0 = range_of(line, x);
-    so0 = b * s.Hkv + g + i0;
-    nown = range_of(line, x + (int64_t)(t_own - 1) * kWOne) - i0 + 1;
-  }
-  const int total = npre * subs + nown * 2;
-  const int cells = G * D4;                    // float4 outputs of the group
-  const int cpb = min(cells, kCombThreads);    // cells per pass
-  const int CG = kCombThreads / cpb;           // thread groups over the pieces
-  const int cg = tid / cpb, ci = tid % cpb;
+  const Pieces q = w.plan[blockIdx.x];
+  const int total = q.n_p + q.n_o;
+#pragma unroll 1
   for (int c0 = 0; c0 < cells; c0 += cpb) {
     const int cell = c0 + ci;
     const bool live = cg < CG && cell < cells;
     const int c4 = live ? cell / G : 0, hh = live ? cell - c4 * G : 0;
     float M = -INFINITY, Ls = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // (m, l) and acc of state (ml, x) into (M, Ls) and acc
+    auto fold = [&](const float2& ml, const float4& x) {
+      if (ml.x == -INFINITY && ml.y == 0.f) return;  // nothing attended: its acc is not written
+      const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+      const float so = fast_exp2(M - ref), sn = fast_exp2(ml.x - ref);
+      acc.x = acc.x * so + x.x * sn;
+      acc.y = acc.y * so + x.y * sn;
+      acc.z = acc.z * so + x.z * sn;
+      acc.w = acc.w * so + x.w * sn;
+      Ls = Ls * so + ml.y * sn;
+      M = mn;
+    };
     constexpr int NU = 4;
+#pragma unroll 1
     for (int k0 = cg; live && k0 < total; k0 += NU * CG) {
       float2 ml[NU];
       float4 x[NU];
@@ -1019,50 +1068,26 @@ __global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const Pref
       for (int u = 0; u < NU; ++u) {
         const int k = k0 + u * CG;
         ml[u] = make_float2(-INFINITY, 0.f);
-        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (k < total) {
-          if (k < npre * subs) {
-            const int64_t state = subs == 2 ? sp0 * 2 + k : (sp0 + k) * 2 + sub0;
-            ml[u] = __ldcg(w.ml_p + state * kT + r0 + hh);
-            x[u] = __ldcg(w.acc_p + (state * D4 + c4) * kT + r0 + hh);
-          } else {
-            const int64_t state = (int64_t)so0 * 2 + (k - npre * subs);
-            ml[u] = __ldcg(w.ml_o + state * G + hh);
-            x[u] = __ldcg(w.acc_o + (state * D4 + c4) * G + hh);
-          }
+          const bool pre = k < q.n_p;
+          const int64_t state = pre ? q.first_p + k * q.stride_p : q.first_o + (k - q.n_p);
+          const int rows = pre ? kT : G, row = pre ? q.r0 + hh : hh;
+          ml[u] = __ldcg((pre ? w.ml_p : w.ml_o) + state * rows + row);
+          x[u] = __ldcg((pre ? w.acc_p : w.acc_o) + (state * D4 + c4) * rows + row);
         }
       }
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
-        if (ml[u].x == -INFINITY && ml[u].y == 0.f) continue;  // nothing attended: acc not written
-        const float mn = fmaxf(M, ml[u].x), ref = mn == -INFINITY ? 0.f : mn;
-        const float so = fast_exp2(M - ref), sn = fast_exp2(ml[u].x - ref);
-        acc.x = acc.x * so + x[u].x * sn;
-        acc.y = acc.y * so + x[u].y * sn;
-        acc.z = acc.z * so + x[u].z * sn;
-        acc.w = acc.w * so + x[u].w * sn;
-        Ls = Ls * so + ml[u].y * sn;
-        M = mn;
-      }
+      for (int u = 0; u < NU; ++u) fold(ml[u], x[u]);
     }
-    __syncthreads();  // the last pass's shared states are read
-    s_acc[tid] = acc;
-    s_ml[tid] = make_float2(M, Ls);
-    __syncthreads();
+    if (CG > 1) {
+      __syncthreads();  // the last pass's shared states are read
+      s_acc[tid] = acc;
+      s_ml[tid] = make_float2(M, Ls);
+      __syncthreads();
+    }
     if (cg == 0 && live) {
-      for (int c = 1; c < CG; ++c) {
-        const float2 ml = s_ml[c * cpb + ci];
-        const float4 x = s_acc[c * cpb + ci];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-        const float so = fast_exp2(M - ref), sn = fast_exp2(ml.x - ref);
-        acc.x = acc.x * so + x.x * sn;
-        acc.y = acc.y * so + x.y * sn;
-        acc.z = acc.z * so + x.z * sn;
-        acc.w = acc.w * so + x.w * sn;
-        Ls = Ls * so + ml.y * sn;
-        M = mn;
-      }
+#pragma unroll 1
+      for (int c = 1; c < CG; ++c) fold(s_ml[c * cpb + ci], s_acc[c * cpb + ci]);
       const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
       // an infinite weight or a NaN anywhere makes this sum NaN or infinite
       if (!(fabsf(acc.x) + fabsf(acc.y) + fabsf(acc.z) + fabsf(acc.w) + fabsf(Ls) < INFINITY))
@@ -1076,7 +1101,7 @@ __global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const Pref
     }
   }
   __syncthreads();
-  for (int hh = tid >> 5; hh < G; hh += kCombThreads / 32)
+  for (int hh = tid >> 5; hh < G; hh += (int)blockDim.x / 32)
     if ((s_bad[hh >> 5] >> (hh & 31)) & 1u) exact_row<T>(p, b, g * G + hh, scale2);
 }
 
@@ -1168,7 +1193,13 @@ int launch_prefix_fast(const PrefixParams& p, int dtype, void* workspace, cudaSt
   else
     rc = bf ? launch_main<128, true>(a, a.masked, stream) : launch_main<128, false>(a, a.masked, stream);
   if (rc) return rc;
-  const dim3 grid((unsigned)(p.B * p.Hkv)), block(kCombThreads);
+  // Threads per unit: one group of threads per unit where the units fill the GPU by themselves, up
+  // to 8 where they do not (a unit then has many states: with few units the prefix is cut finely).
+  const int cells = (int)(p.G * p.D / 4);
+  const int64_t units = p.B * p.Hkv;
+  const int groups = units >= 1024 ? 1 : units >= 512 ? 2 : units >= 256 ? 4 : 8;
+  const int threads = std::min(kCombThreads, (std::min(cells, kCombThreads) * groups + 31) / 32 * 32);
+  const dim3 grid((unsigned)units), block((unsigned)threads);
   if (bf)
     return launch_dependent(prefix_combine_kernel<__nv_bfloat16>, grid, block, 0, stream, "prefix_combine_kernel", p, a.s,
                             a.w, a.scale2);

@@ -363,9 +363,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       mbar_init(&bars[L::bQFull + i], 1);
       mbar_init(&bars[L::bQEmpty + i], 1);
       mbar_init(&bars[L::bSFull + i], 1);
-      mbar_init(&bars[L::bPFull + i], kGroupThreads);
+      mbar_init(&bars[L::bPFull + i], 4);  // the group's warps
       mbar_init(&bars[L::bODone + i], 1);
-      mbar_init(&bars[L::bOFree + i], kGroupThreads);
+      mbar_init(&bars[L::bOFree + i], 4);
     }
     for (int i = 0; i < L::kDescs; ++i) {
       mbar_init(&bars[L::bDFull + i], 1);
@@ -626,128 +626,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
         ++d;
       }
-    } else if (warp == kMmaWarp) {
-      // ---------------------------------------------------------------- MMA issuer (one thread)
-      if (elect_one()) {
-      const int dk = (S.D + 15) / 16;  // K steps of Q K^T, and N / 16 of P V
-      const uint32_t id_pv = idesc_f16(kT, dk * 16, BF16, false, true);
-      struct Job {
-        uint32_t tile;  // key tile index: K in ring entry 2 tile, V in 2 tile + 1
-        int vr;
-        uint32_t bits;  // lane | J_*
-      };
-      enum : uint32_t { J_FIRST = 2, J_LAST = 4, J_REL = 8 };
-      Job j0{}, j1{};  // pending P V products, j0 the older
-      int np = 0;
-      uint32_t d = 0, tile = 0, job = 0, nq = 0, pc[2] = {0, 0}, of[2] = {0, 0};
-      int in_item = 0;          // key tiles of the item so far
-      int left = 0, rts = 0;    // row tiles of the current key tile still to multiply, of how many
-      int flags = 0, vr = 0;
-      bool flush = false;
-      // One product per turn, P V of the older pending job as soon as two are pending (its P is
-      // then due first), else Q K^T of the next.
-      while (true) {
-        if (np == 2 || (flush && np > 0)) {
-          // ---- O[g] += P V
-          const uint32_t g = j0.bits & 1u;
-          const uint32_t seq = 2 * j0.tile + 1, sl = seq % L::kSlots;
-          if (j0.bits & J_FIRST) {  // O[g] has been read by the last item's epilogue
-            if (!mbar_wait(&bars[L::bOFree + g], ((g ? of[1] : of[0]) & 1) ^ 1, st)) break;
-            if (g) ++of[1]; else ++of[0];
-          }
-          if (!mbar_wait(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
-          const int n16 = (j0.vr + 15) & ~15;
-          if (!mbar_wait(&bars[L::bPFull + g], (g ? pc[1] : pc[0]) & 1, st)) break;
-          if (g) ++pc[1]; else ++pc[0];
-          {
-            tc_fence_after();
-            const uint64_t vd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), kT * 128, 1024);
-            const uint32_t d_o = tmem + kColO + g * kT, a_p = tmem + kColS + g * kT;
-            const uint32_t acc = (j0.bits & J_FIRST) ? 0u : 1u;
-#pragma unroll
-            for (int kk = 0; kk < kT / 16; ++kk)
-              if (kk * 16 < n16)
-                tc_mma_f16_ts(d_o, a_p + kk * 8, desc_add(vd, kk * 16 * 128), id_pv, kk > 0 ? 1u : acc);
-            if (j0.bits & J_REL) tc_commit(&bars[L::bEmpty + sl]);
-            if (j0.bits & J_LAST) tc_commit(&bars[L::bODone + g]);
-          }
-          j0 = j1;
-          --np;
-          continue;
-        }
-        if (flush) {
-          if (flags & F_END) break;
-          flush = false;
-        }
-        if (left == 0) {
-          // ---- the next key tile
-          const uint32_t ds = d % L::kDescs;
-          if (!mbar_wait(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
-          flags = descs[ds].flags;
-          vr = descs[ds].vr;
-          // at the end, and where an item has nothing to multiply, finish what is pending: the softmax
-          // groups wait for their last item's accumulators before they release more descriptors
-          flush = flags & (F_END | F_EMPTY);
-          if (!(flags & F_END)) mbar_arrive(&bars[L::bDEmpty + ds]);
-          ++d;
-          if (flush) continue;
-          rts = left = flags & F_PAIR ? 2 : 1;
-          if (flags & F_FIRST) {
-            in_item = 0;
-            if (!mbar_wait(&bars[L::bQFull + (nq & 1)], (nq >> 1) & 1, st)) break;
-            if (rts == 2 && !mbar_wait(&bars[L::bQFull + ((nq + 1) & 1)], ((nq + 1) >> 1) & 1, st)) break;
-          }
-          if (!mbar_wait(&bars[L::bFull + (2 * tile) % L::kSlots], ((2 * tile) / L::kSlots) & 1, st)) break;
-        }
-        // ---- S[g] = Q K^T
-        const uint32_t g = job & 1, sl = (2 * tile) % L::kSlots, qb = (nq + rts - left) & 1;
-        {
-          tc_fence_after();
-          const uint32_t id_qk = idesc_f16(kT, (vr + 15) & ~15, BF16, false, false);
-          const uint64_t qd = smem_desc(smem_u32(sm + L::kQ + qb * L::kTile), 16, 1024);
-          const uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
-          const uint32_t d_s = tmem + kColS + g * kT;
-#pragma unroll
-          for (int kk = 0; kk < DT / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
-            if (kk < dk) tc_mma_f16(d_s, desc_add(qd, off), desc_add(kd, off), id_qk, kk > 0 ? 1u : 0u);
-          }
-          tc_commit(&bars[L::bSFull + g]);
-          if (left == 1) tc_commit(&bars[L::bEmpty + sl]);
-          if (flags & F_LAST) tc_commit(&bars[L::bQEmpty + qb]);
-        }
-        // the lane's first product of the item: its first tile's, or, where the lanes take the tiles in
-        // turn, its second tile's
-        Job j;
-        j.tile = tile;
-        j.vr = vr;
-        j.bits = g | ((in_item == 0 || (rts == 1 && in_item == 1)) ? J_FIRST : 0u) | ((flags & F_LAST) ? J_LAST : 0u) |
-                 (left == 1 ? J_REL : 0u);
-        if (rts == 1 && (flags & F_LAST) && in_item > 0) j0.bits |= J_LAST;  // the other lane's last, still pending
-        if (np == 0) j0 = j; else j1 = j;
-        ++np;
-        ++job;
-        if (--left == 0) {
-          ++tile;
-          ++in_item;
-          if (flags & F_LAST) nq += rts;
-        }
-      }
-      }
-    }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    // ------------------------------------------------------------------ softmax warpgroups
-    const int grp = warp >> 2, quarter = warp & 3;
-    const int rl = quarter * 32 + lane;  // row of the tile == TMEM lane
-    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t col_s = kColS + grp * kT, col_o = kColO + grp * kT;
-    const float sc2 = a.scale2;
-    const int G = S.G, D4 = S.D / 4;
-    if (warp == 4) {
-      // Before its first scores arrive, this warp writes down for the join where the partial states of
-      // the CTA's share of the requests are (lane = KV head): the CTAs whose ranges hold the first and
-      // last tile of the prefix unit and of the own unit.
+    } else if (warp == kTmemWarp) {
+      // ---------------------------------------------------------------- plan of the join
+      // Where the partial states of the CTA's share of the requests are (lane = KV head): the CTAs
+      // whose ranges hold the first and last tile of the prefix unit and of the own unit.
       const int per = (S.B + (int)gridDim.x - 1) / (int)gridDim.x;
       const int ba = min(S.B, (int)blockIdx.x * per), bz = min(S.B, ba + per);
       int cum = 0;
@@ -764,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         const bool pr = rt < 2 * pairs;
 #pragma unroll 1
         for (int g = lane; g < S.Hkv; g += 32) {
-          Pieces q{0, 0, pr ? 2 : 1, (b - rt * S.nb) * G, 0, 0, {0, 0}};
+          Pieces q{0, 0, pr ? 2 : 1, (b - rt * S.nb) * S.G, 0, 0, {0, 0}};
           if (line.tiles_p > 0) {
             const int u = pr ? g * pairs + rt / 2 : S.units[0] + g, wt = pr ? kWPair : kWOne;
             const int64_t x = pr ? (int64_t)u * line.tiles_p * kWPair : line.len[0] + (int64_t)g * line.tiles_p * kWOne;
@@ -782,8 +664,143 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         }
         cum += t;
       }
-      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------------- MMA issuer (one thread)
+      if (elect_one()) {
+      const int dk = (S.D + 15) / 16;  // K steps of Q K^T, and N / 16 of P V
+      const uint32_t id_pv = idesc_f16(kT, dk * 16, BF16, false, true);
+      struct Job {
+        uint32_t tile;  // key tile index: K in ring entry 2 tile, V in 2 tile + 1
+        int vr;
+        uint32_t bits;  // lane | J_*
+      };
+      enum : uint32_t { J_FIRST = 2, J_LAST = 4, J_REL = 8 };
+      Job j0{}, j1{};  // pending P V products, j0 the older
+      int np = 0;
+      uint32_t d = 0, tile = 0, job = 0, nq = 0, pc[2] = {0, 0}, of[2] = {0, 0};
+int in_item = 0;          // key tiles of the item so far
+      int left = 0, rts = 0;    // row tiles of the current key tile still to multiply, of how many
+      int flags = 0, vr = 0, stage = 0;
+      bool flush = false;
+      long long idle = clock64();
+      // Polls what it may do next: a pending P V once its P is there (at the latest before the Q K^T
+      // that reuses its lane), and meanwhile the next key tile's descriptor, Q and K, so that
+      // the lane's next Q K^T follows its P V at once.
+      while (true) {
+        bool busy = false;
+        // ---- the next key tile: descriptor, then Q of a new item, then K
+        if (stage == 0 && !flush && mbar_test(&bars[L::bDFull + d % L::kDescs], (d / L::kDescs) & 1)) {
+          const uint32_t ds = d % L::kDescs;
+          flags = descs[ds].flags;
+          vr = descs[ds].vr;
+          // at the end, and where an item has nothing to multiply, finish what is pending: the softmax
+          // groups wait for their last item's accumulators before they release more descriptors
+          flush = flags & (F_END | F_EMPTY);
+          if (!(flags & F_END)) mbar_arrive(&bars[L::bDEmpty + ds]);
+          ++d;
+          if (!flush) {
+            rts = flags & F_PAIR ? 2 : 1;
+            stage = flags & F_FIRST ? 1 : 2;
+            if (flags & F_FIRST) in_item = 0;
+          }
+          busy = true;
+        }
+        if (stage == 1 && mbar_test(&bars[L::bQFull + (nq & 1)], (nq >> 1) & 1) &&
+            (rts == 1 || mbar_test(&bars[L::bQFull + ((nq + 1) & 1)], ((nq + 1) >> 1) & 1)))
+          stage = 2;
+        if (stage == 2 && mbar_test(&bars[L::bFull + (2 * tile) % L::kSlots], ((2 * tile) / L::kSlots) & 1)) {
+          stage = 3;
+          left = rts;
+          busy = true;
+        }
+        const uint32_t pg = j0.bits & 1u, pph = (pg ? pc[1] : pc[0]) & 1;
+        // nothing else to do before the older pending P arrives: wait for it
+        if (np == 2 && stage == 3 && !mbar_wait(&bars[L::bPFull + pg], pph, st)) break;
+        if (np > 0 && (np == 2 || stage != 3) && mbar_test(&bars[L::bPFull + pg], pph)) {
+          // ---- O[g] += P V
+          const uint32_t g = pg;
+          const uint32_t seq = 2 * j0.tile + 1, sl = seq % L::kSlots;
+          if (j0.bits & J_FIRST) {  // O[g] has been read by the last item's epilogue
+            if (!mbar_wait(&bars[L::bOFree + g], ((g ? of[1] : of[0]) & 1) ^ 1, st)) break;
+            if (g) ++of[1]; else ++of[0];
+          }
+          if (!mbar_wait(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
+          const int n16 = (j0.vr + 15) & ~15;
+          if (g) ++pc[1]; else ++pc[0];
+          tc_fence_after();
+          const uint64_t vd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), kT * 128, 1024);
+          const uint32_t d_o = tmem + kColO + g * kT, a_p = tmem + kColS + g * kT;
+          const uint32_t acc = (j0.bits & J_FIRST) ? 0u : 1u;
+#pragma unroll
+          for (int kk = 0; kk < kT / 16; ++kk)
+            if (kk * 16 < n16)
+              tc_mma_f16_ts(d_o, a_p + kk * 8, desc_add(vd, kk * 16 * 128), id_pv, kk > 0 ? 1u : acc);
+          if (j0.bits & J_REL) tc_commit(&bars[L::bEmpty + sl]);
+          if (j0.bits & J_LAST) tc_commit(&bars[L::bODone + g]);
+          j0 = j1;
+          --np;
+          busy = true;
+        } else if (flush && np == 0) {
+          if (flags & F_END) break;
+          flush = false;
+        }
+        if (stage == 3 && np < 2) {
+          // ---- S[g] = Q K^T
+          const uint32_t g = job & 1, sl = (2 * tile) % L::kSlots, qb = (nq + rts - left) & 1;
+          tc_fence_after();
+          const uint32_t id_qk = idesc_f16(kT, (vr + 15) & ~15, BF16, false, false);
+          const uint64_t qd = smem_desc(smem_u32(sm + L::kQ + qb * L::kTile), 16, 1024);
+          const uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
+          const uint32_t d_s = tmem + kColS + g * kT;
+#pragma unroll
+          for (int kk = 0; kk < DT / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
+            if (kk < dk) tc_mma_f16(d_s, desc_add(qd, off), desc_add(kd, off), id_qk, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(&bars[L::bSFull + g]);
+          if (left == 1) tc_commit(&bars[L::bEmpty + sl]);
+          if (flags & F_LAST) tc_commit(&bars[L::bQEmpty + qb]);
+          // the lane's first product of the item: its first tile's, or, where the lanes take the tiles
+          // in turn, its second tile's
+          Job j;
+          j.tile = tile;
+          j.vr = vr;
+          j.bits = g | ((in_item == 0 || (rts == 1 && in_item == 1)) ? J_FIRST : 0u) | ((flags & F_LAST) ? J_LAST : 0u) |
+                   (left == 1 ? J_REL : 0u);
+          if (rts == 1 && (flags & F_LAST) && in_item > 0) {
+            // the other lane's last product of the item is the one before this: pending, or issued
+            if (np > 0) j0.bits |= J_LAST;
+            else tc_commit(&bars[L::bODone + (g ^ 1)]);
+          }
+          if (np == 0) j0 = j; else j1 = j;
+          ++np;
+          ++job;
+          if (--left == 0) {
+            stage = 0;
+            ++tile;
+            ++in_item;
+            if (flags & F_LAST) nq += rts;
+          }
+          busy = true;
+        }
+        if (busy) {
+          idle = clock64();
+        } else if (clock64() - idle > (1ll << 31)) {
+          raise_status(st, kStatusWaitTimeout);
+          break;
+        }
+      }
+      }
     }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------------------------ softmax warpgroups
+    const int grp = warp >> 2, quarter = warp & 3;
+    const int rl = quarter * 32 + lane;  // row of the tile == TMEM lane
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t col_s = kColS + grp * kT, col_o = kColO + grp * kT;
+    const float sc2 = a.scale2;
+    const int G = S.G, D4 = S.D / 4;
     uint32_t d = 0, job = 0, tile = 0, sc = 0, od = 0;
     float m_used = -INFINITY, l_sum = 0.f;
     bool had = false;
@@ -824,98 +841,146 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         if (!mbar_wait_warp(&bars[L::bSFull + grp], sc & 1, st)) break;
         ++sc;
         tc_fence_after();
+        uint64_t ls = 0;
+        float la = 1.f;  // the sum's rescale
         if (__any_sync(0xffffffffu, row_ok)) {
-          const int nch = (vr + 31) >> 5;  // 32-key chunks with valid keys
-          if (vr & 31) {
-            // the last chunk's columns past the valid keys hold whatever was there: -inf in place
-            float x[32];
-            tmem_ld32(lane_addr + col_s + (nch - 1) * 32, x);
-            tmem_wait_ld();
+          bool done = false;
+          if (vr == kT && !own) {
+            // Full prefix tile, one pass: the reference stays what it is (0 in the row's first tile), and nothing
+            // needs the maximum as long as the exponentials' sum tells that none overflowed and, in a
+            // first tile, that the row's largest is not lost in the type's small numbers: within
+            // [1, 2^13] the largest of 128 is at least 2^-7, and fp16 holds 2^13.  Any row outside (or a
+            // NaN) sends the warp through the two-pass form below; P is kept in registers till then, as
+            // it overwrites S.  (Own items are short and wait for memory: there the two-pass form, whose
+            // loops are a third of this code, measured faster, 127 against 141 us at 256 requests of
+            // up to 768 tokens; over the prefix one pass takes 1.6 k cycles a tile, two take 2.7 k.)
+            const float ref = m_used == -INFINITY ? 0.f : m_used;
+            const uint64_t scale_x2 = f32x2(sc2, sc2);
+            uint64_t rs[2] = {0, 0};
+            uint32_t pk[kT / 2];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = i < (vr & 31) ? x[i] : -INFINITY;
-            tmem_st32(lane_addr + col_s + (nch - 1) * 32, x);
-            tmem_wait_st();
-          }
-          // Row maximum, per group of 8 keys so that a masked group falls away by selection.
-          float mraw = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < nch; c += 2) {
-            float x[64];
-            tmem_ld32(lane_addr + col_s + c * 32, reinterpret_cast<float(&)[32]>(x[0]));
-            if (c + 1 < nch) tmem_ld32(lane_addr + col_s + c * 32 + 32, reinterpret_cast<float(&)[32]>(x[32]));
-            tmem_wait_ld();
-            const int nk = c + 1 < nch ? 8 : 4;
+            for (int half = 0; half < 2; ++half) {
+              float x[2][32];
+              tmem_ld32(lane_addr + col_s + half * 64, x[0]);
+              tmem_ld32(lane_addr + col_s + half * 64 + 32, x[1]);
+              tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float* y = x + 8 * k;
-              const float mg = fmax3(fmax3(y[0], y[1], y[2]), fmax3(y[3], y[4], y[5]), fmaxf(y[6], y[7]));
-              if (k < nk) mraw = fmaxf(mraw, (gm >> (c * 4 + k)) & 1u ? mg : -INFINITY);
+              for (int k = 0; k < 8; ++k) {
+                const float bk = (gm >> (half * 8 + k)) & 1u ? -ref : -INFINITY;
+                const uint64_t bias_x2 = f32x2(bk, bk);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                  float e0, e1;
+                  const float* y = &x[k >> 2][(k & 3) * 8 + i];
+                  f32x2_split(fma_f32x2(f32x2(y[0], y[1]), scale_x2, bias_x2), e0, e1);
+                  const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
+                  rs[(i >> 1) & 1] = add_f32x2(rs[(i >> 1) & 1], f32x2(p0, p1));
+                  pk[half * 32 + k * 4 + i / 2] = pack2(p0, p1, BF16);
+                }
+              }
+              // the first half's columns end here: loaded any earlier, the second half's would push
+              // the warp past its registers
+#pragma unroll
+              for (int i = 0; i < 32; i += 8)
+                asm volatile("" ::"r"(pk[half * 32 + i]), "r"(pk[half * 32 + i + 1]), "r"(pk[half * 32 + i + 2]),
+                             "r"(pk[half * 32 + i + 3]), "r"(pk[half * 32 + i + 4]), "r"(pk[half * 32 + i + 5]),
+                             "r"(pk[half * 32 + i + 6]), "r"(pk[half * 32 + i + 7]));
+            }
+            ls = add_f32x2(rs[0], rs[1]);
+            float r0, r1;
+            f32x2_split(ls, r0, r1);
+            const float sum = r0 + r1;
+            done = __all_sync(0xffffffffu, gm == 0u || (sum <= 8192.f && (m_used != -INFINITY || sum >= 1.f)));
+            if (done) {
+#pragma unroll
+              for (int c = 0; c < kT / 32; ++c) tmem_st16(lane_addr + col_s + c * 16, pk + c * 16);
+              if (gm != 0u) m_used = ref;
             }
           }
-          const float mt = mraw * sc2;
-          float m_new = m_used;
-          if (mt > -INFINITY && (m_used == -INFINITY || mt > m_used + kRescaleThreshold)) m_new = mt;
-          const float m_ref = m_new == -INFINITY ? 0.f : m_new;
-          const float alpha = m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_ref);
-          const bool rescale = m_new != m_used && m_used != -INFINITY;
-          const uint64_t scale_x2 = f32x2(sc2, sc2);
-          uint64_t rs0 = 0, rs1 = 0;
-          // Exponentials and P, 32 keys at a time from a second read of S: a loop this short stays in
-          // the instruction cache beside the MMA warp's code, which the 128 unrolled columns of a
-          // single read evict.  A masked group's bias is -inf.
-          float xa[32], xb[32];
-          auto chunk = [&](const float(&x)[32], int c) {
-            uint32_t pk[16];
+          if (__builtin_expect(!done, 0)) {
+            const int nch = (vr + 31) >> 5;  // 32-key chunks with valid keys
+            if (vr & 31) {
+              // the last chunk's columns past the valid keys hold whatever was there: -inf in place
+              float x[32];
+              tmem_ld32(lane_addr + col_s + (nch - 1) * 32, x);
+              tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float bk = (gm >> (c * 4 + k)) & 1u ? -m_ref : -INFINITY;
-              const uint64_t bias_x2 = f32x2(bk, bk);
+              for (int i = 0; i < 32; ++i) x[i] = i < (vr & 31) ? x[i] : -INFINITY;
+              tmem_st32(lane_addr + col_s + (nch - 1) * 32, x);
+              tmem_wait_st();
+            }
+            // Row maximum, per group of 8 keys so that a masked group falls away by selection.
+            float mraw = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < nch; c += 2) {
+              float x[64];
+              tmem_ld32(lane_addr + col_s + c * 32, reinterpret_cast<float(&)[32]>(x[0]));
+              if (c + 1 < nch) tmem_ld32(lane_addr + col_s + c * 32 + 32, reinterpret_cast<float(&)[32]>(x[32]));
+              tmem_wait_ld();
+              const int nk = c + 1 < nch ? 8 : 4;
 #pragma unroll
-              for (int i = k * 8; i < k * 8 + 8; i += 2) {
-                float e0, e1;
-                f32x2_split(fma_f32x2(f32x2(x[i], x[i + 1]), scale_x2, bias_x2), e0, e1);
-                const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
-                if (i & 2) rs1 = add_f32x2(rs1, f32x2(p0, p1));
-                else rs0 = add_f32x2(rs0, f32x2(p0, p1));
-                pk[i / 2] = pack2(p0, p1, BF16);
+              for (int k = 0; k < 8; ++k) {
+                const float* y = x + 8 * k;
+                const float mg = fmax3(fmax3(y[0], y[1], y[2]), fmax3(y[3], y[4], y[5]), fmaxf(y[6], y[7]));
+                if (k < nk) mraw = fmaxf(mraw, (gm >> (c * 4 + k)) & 1u ? mg : -INFINITY);
               }
             }
-            tmem_st16(lane_addr + col_s + c * 16, pk);
-          };
-          tmem_ld32(lane_addr + col_s, xa);
-          tmem_wait_ld();
-#pragma unroll 1
-          for (int c = 0; c < nch; c += 2) {
-            const bool two = c + 1 < nch;
-            if (two) tmem_ld32(lane_addr + col_s + c * 32 + 32, xb);
-            chunk(xa, c);
-            if (two) {
-              tmem_wait_ld();
-              if (c + 2 < nch) tmem_ld32(lane_addr + col_s + c * 32 + 64, xa);
-              chunk(xb, c + 1);
-              tmem_wait_ld();
-            }
-          }
-          // S(i) being complete implies that the lane's last P V is: O[g] may be rescaled here
-          if (had && __any_sync(0xffffffffu, rescale)) {
-            const float f = rescale ? alpha : 1.f;
-#pragma unroll 1
-            for (int c = 0; c < DT / 32; ++c) {
-              float o[32];
-              tmem_ld32(lane_addr + col_o + c * 32, o);
-              tmem_wait_ld();
+            const float mt = mraw * sc2;
+            float m_new = m_used;
+            if (mt > -INFINITY && (m_used == -INFINITY || mt > m_used + kRescaleThreshold)) m_new = mt;
+            const float m_ref = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = m_used == -INFINITY ? 1.f : fast_exp2(m_used - m_ref);
+            const bool rescale = m_new != m_used && m_used != -INFINITY;
+            const uint64_t scale_x2 = f32x2(sc2, sc2);
+            uint64_t rs0 = 0, rs1 = 0;
+            // Exponentials and P, 32 keys at a time from a second read of S: a loop this short stays in
+            // the instruction cache beside the MMA warp's code, which the 128 unrolled columns of a
+            // single read evict.  A masked group's bias is -inf.
+            auto chunk = [&](const float(&x)[32], int c) {
+              uint32_t pk[16];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= f;
-              tmem_st32(lane_addr + col_o + c * 32, o);
+              for (int k = 0; k < 4; ++k) {
+                const float bk = (gm >> (c * 4 + k)) & 1u ? -m_ref : -INFINITY;
+                const uint64_t bias_x2 = f32x2(bk, bk);
+#pragma unroll
+                for (int i = k * 8; i < k * 8 + 8; i += 2) {
+                  float e0, e1;
+                  f32x2_split(fma_f32x2(f32x2(x[i], x[i + 1]), scale_x2, bias_x2), e0, e1);
+                  const float p0 = fast_exp2(e0), p1 = fast_exp2(e1);
+                  if (i & 2) rs1 = add_f32x2(rs1, f32x2(p0, p1));
+                  else rs0 = add_f32x2(rs0, f32x2(p0, p1));
+                  pk[i / 2] = pack2(p0, p1, BF16);
+                }
+              }
+              tmem_st16(lane_addr + col_s + c * 16, pk);
+            };
+#pragma unroll 1
+            for (int c = 0; c < nch; ++c) {
+              float x[32];
+              tmem_ld32(lane_addr + col_s + c * 32, x);
+              tmem_wait_ld();
+              chunk(x, c);
             }
+            // S(i) being complete implies that the lane's last P V is: O[g] may be rescaled here
+            if (had && __any_sync(0xffffffffu, rescale)) {
+              const float f = rescale ? alpha : 1.f;
+#pragma unroll 1
+              for (int c = 0; c < DT / 32; ++c) {
+                float o[32];
+                tmem_ld32(lane_addr + col_o + c * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= f;
+                tmem_st32(lane_addr + col_o + c * 32, o);
+              }
+            }
+            ls = add_f32x2(rs0, rs1);
+            la = m_used == -INFINITY ? 0.f : alpha;
+            m_used = m_new;
           }
           tmem_wait_st();
-          float r0, r1;
-          f32x2_split(add_f32x2(rs0, rs1), r0, r1);
-          l_sum = (m_used == -INFINITY ? 0.f : l_sum * alpha) + (r0 + r1);
-          m_used = m_new;
         }
-        if (vr & 15) {
+        if (__builtin_expect(vr & 15, 0)) {
           // V rows past the valid keys meet P = 0 in the product's last K step: they must be finite, so
           // they are cleared (in a pair tile by both groups, with the same zeros)
           const uint32_t seq = 2 * (tile - 1) + 1, sl = seq % L::kSlots;
@@ -930,7 +995,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           fence_proxy_async_smem();
         }
         tc_fence_before();
-        mbar_arrive(&bars[L::bPFull + grp]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[L::bPFull + grp]);
+        float r0, r1;
+        f32x2_split(ls, r0, r1);
+        l_sum = fmaf(l_sum, la, r0 + r1);
         had = true;
       }
       if (!(flags & F_LAST)) continue;
@@ -958,7 +1027,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           }
         }
         tc_fence_before();
-        mbar_arrive(&bars[L::bOFree + grp]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[L::bOFree + grp]);
       }
     }
   }

@@ -1188,7 +1188,12 @@ int launch_main(const Args& a, bool dependent, cudaStream_t stream) {
   if (regs != kLaunchRegs)
     return fail(SA_ELAUNCH, "prefix decode: launch register count " + std::to_string(regs) +
                                 " differs from the register split's " + std::to_string(kLaunchRegs));
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DT>::kAlloc);
+  static bool opted[64] = {};  // per device; setting it again is harmless
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !opted[dev]) {
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<DT>::kAlloc);
+    if (dev >= 0 && dev < 64) opted[dev] = true;
+  }
   if (dependent)
     return launch_dependent(kern, dim3(a.s.grid), dim3(kThreads), Layout<DT>::kAlloc, stream, "prefix_sm100_kernel", a);
   kern<<<a.s.grid, kThreads, Layout<DT>::kAlloc, stream>>>(a);

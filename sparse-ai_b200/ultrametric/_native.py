@@ -36,19 +36,19 @@ _SIGNATURES = {
     "sa_paged_kv_append": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _vp, _p64, _vp, _p64, _vp,
                                    _p64, _i64, _vp, _vp, _p64, _vp, _p64, _vp, _i32, _p64, _i64,
                                    _i64, _vp, _i32, _p64, _vp]),
-    "sa_paged_build_tables": (_i32, [_i64, _i64, _i64, _i64, _vp, _vp, _vp, _p64, _vp, _i64, _vp,
+    "sa_paged_build_tables": (_i32, [_i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp,
                                      _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "sa_paged_release": (_i32, [_i64, _i64, _i64, _vp, _vp, _vp, _p64, _vp, _i64, _vp, _vp, _vp,
+    "sa_paged_release": (_i32, [_i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp,
                                 _vp]),
-    "sa_paged_kv_write": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _vp, _p64, _vp, _p64, _vp,
-                                 _vp, _p64, _vp, _p64, _vp, _i32, _p64, _i64, _i64, _vp, _i32,
-                                 _p64, _vp]),
+    "sa_paged_kv_write": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp,
+                                 _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _vp, _i32,
+                                 _vp, _vp]),
     "sa_ultrametric_prefix_decode_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64,
                                                             _i64, _i64]),
-    "sa_ultrametric_prefix_decode": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _p64,
-                                            _vp, _p64, _vp, _p64, _vp, _i64, _i64, _vp, _vp, _p64,
-                                            _i64, _vp, _vp, _i32, _p64, _vp, _i32, _p64, _i64,
-                                            _i64, _i64, _i32, _vp, _p64, _vp, _vp, _i64, _vp]),
+    "sa_ultrametric_prefix_decode": (_i32, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
+                                            _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp,
+                                            _i64, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64,
+                                            _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
     "sa_ternary_quantize_pack": (_i32, [_i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
     "sa_ternary_dequantize": (_i32, [_i32, _i64, _i64, _vp, _vp, _vp, _i64, _vp]),
     "sa_build_block_lists_from_assignments": (_i32, [_vp, _i32, _p64, _i64, _i64, _i64, _i64,
@@ -130,6 +130,20 @@ def strides(t: torch.Tensor, ndim: int | None = None):
     return (ctypes.c_int64 * len(st))(*st)
 
 
+_STRIDE_ARRAYS = {}  # stride tuple -> (array, its address); kept for the process
+
+
+def cached_strides(t: torch.Tensor) -> int:
+    """Address of an int64 array of the tensor's strides, one per distinct stride tuple (the library
+    only reads it): building and converting one takes about 1 us, as much as a launch argument list."""
+    st = t.stride()
+    e = _STRIDE_ARRAYS.get(st)
+    if e is None:
+        a = (ctypes.c_int64 * len(st))(*st)
+        e = _STRIDE_ARRAYS[st] = (a, ctypes.addressof(a))
+    return e[1]
+
+
 def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -148,6 +162,14 @@ def int_code(dtype: torch.dtype) -> int:
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(t: torch.Tensor) -> int:
+    """``stream_of`` without building a Stream object (about 1 us less per call)."""
+    return _raw_stream(t.get_device()) if _raw_stream is not None else stream_of(t)
 
 
 def require_cuda(name: str, *tensors) -> None:

@@ -11,11 +11,17 @@ on the joined page list, as if the prefix's pages stood first in every block tab
 
 from __future__ import annotations
 
+import functools
 from typing import Union
 
 import torch
 
 from . import _native as nat
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(code, B, H, Hkv, D, page, Lp, L, device_index):
+    return max(256, int(nat.lib().sa_ultrametric_prefix_decode_workspace_bytes(code, B, H, Hkv, D, page, Lp, L)))
 
 
 def ultrametric_prefix_decode(
@@ -58,11 +64,11 @@ def ultrametric_prefix_decode(
     if not (q.dtype == k_cache.dtype == v_cache.dtype):
         raise ValueError("q, k_cache, v_cache must share dtype")
     if prefix_pages.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != B or \
-            tuple(context_lens.shape) != (B,):
+            context_lens.shape != (B,):
         raise ValueError(f"expected prefix_pages (Lp,), block_tables ({B}, L) and context_lens ({B},); got "
                          f"{tuple(prefix_pages.shape)}, {tuple(block_tables.shape)}, {tuple(context_lens.shape)}")
-    if router_indices.dim() != 3 or tuple(router_indices.shape[:2]) != (P, H) or \
-            q_router_indices.dim() != 3 or tuple(q_router_indices.shape[:2]) != (B, H) or \
+    if router_indices.dim() != 3 or router_indices.shape[:2] != (P, H) or \
+            q_router_indices.dim() != 3 or q_router_indices.shape[:2] != (B, H) or \
             q_router_indices.shape[2] < 1 or router_indices.shape[2] != q_router_indices.shape[2]:
         raise ValueError(f"router_indices must be ({P}, {H}, TD) and q_router_indices ({B}, {H}, TD); got "
                          f"{tuple(router_indices.shape)}, {tuple(q_router_indices.shape)}")
@@ -83,24 +89,23 @@ def ultrametric_prefix_decode(
     nat.require_cuda("ultrametric_prefix_decode", q, k_cache, v_cache, prefix_pages, plen_dev, block_tables,
                      context_lens, router_indices, q_router_indices)
     code = nat.float_code(q.dtype)
-    pp = prefix_pages.to(torch.int32).contiguous()
-    bt = block_tables.to(torch.int32)
-    ctx = context_lens.to(torch.int32).contiguous()
-    ri = router_indices if router_indices.dtype in (torch.int32, torch.int64) else router_indices.to(torch.int64)
-    qri = q_router_indices if q_router_indices.dtype in (torch.int32, torch.int64) else q_router_indices.to(torch.int64)
+    i32, i64 = torch.int32, torch.int64
+    pp = (prefix_pages if prefix_pages.dtype is i32 else prefix_pages.to(i32)).contiguous()
+    bt = block_tables if block_tables.dtype is i32 else block_tables.to(i32)
+    ctx = (context_lens if context_lens.dtype is i32 else context_lens.to(i32)).contiguous()
+    ri = router_indices if router_indices.dtype in (i32, i64) else router_indices.to(i64)
+    qri = q_router_indices if q_router_indices.dtype in (i32, i64) else q_router_indices.to(i64)
     kc = k_cache if k_cache.stride(-1) == 1 else k_cache.contiguous()
     vc = v_cache if v_cache.stride(-1) == 1 else v_cache.contiguous()
     qq = q if q.stride(-1) == 1 else q.contiguous()
     out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H), dtype=torch.float32, device=q.device) if return_lse else None
-    Lp, L = pp.shape[0], bt.shape[1]
-    ws_bytes = int(nat.lib().sa_ultrametric_prefix_decode_workspace_bytes(code, B, H, Hkv, D, page, Lp, L))
-    ws = torch.empty(max(ws_bytes, 256), dtype=torch.uint8, device=q.device)
+    Lp, L, st = pp.shape[0], bt.shape[1], nat.cached_strides
+    ws_bytes = _workspace_bytes(code, B, H, Hkv, D, page, Lp, L, q.get_device())
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     nat.check(nat.lib().sa_ultrametric_prefix_decode(
-        code, B, H, Hkv, D, page, P, qq.data_ptr(), nat.strides(qq), kc.data_ptr(), nat.strides(kc),
-        vc.data_ptr(), nat.strides(vc), pp.data_ptr(), Lp, plen, nat.ptr(plen_dev), bt.data_ptr(), nat.strides(bt), L,
-        ctx.data_ptr(), ri.data_ptr(), nat.int_code(ri.dtype), nat.strides(ri), qri.data_ptr(),
-        nat.int_code(qri.dtype), nat.strides(qri), TD, int(req_depth), int(local_blocks), int(bool(sink_block)),
-        out.data_ptr(), nat.strides(out), nat.ptr(lse), ws.data_ptr(), ws.numel(), nat.stream_of(q)),
-        "ultrametric_prefix_decode")
+        code, B, H, Hkv, D, page, P, qq.data_ptr(), st(qq), kc.data_ptr(), st(kc), vc.data_ptr(), st(vc), pp.data_ptr(), Lp,
+        plen, nat.ptr(plen_dev), bt.data_ptr(), st(bt), L, ctx.data_ptr(), ri.data_ptr(), nat.int_code(ri.dtype), st(ri),
+        qri.data_ptr(), nat.int_code(qri.dtype), st(qri), TD, int(req_depth), int(local_blocks), int(bool(sink_block)),
+        out.data_ptr(), st(out), nat.ptr(lse), ws.data_ptr(), ws_bytes, nat.raw_stream(q)), "ultrametric_prefix_decode")
     return (out, lse) if return_lse else out

@@ -45,7 +45,7 @@ class PagedTables(NamedTuple):
 
 
 def _int32(name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
-    if t.dtype != torch.int32 or tuple(t.shape) != shape:
+    if t.dtype is not torch.int32 or t.shape != shape:
         raise ValueError(f"{name} must be int32 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     return t
 
@@ -67,7 +67,6 @@ def _tables_args(context_lens, block_tables, free_pages, num_free, page_size):
     return B, L
 
 
-@torch.no_grad()
 def build_paged_tables(
     context_lens: torch.Tensor,
     new_lens: torch.Tensor,
@@ -103,18 +102,21 @@ def build_paged_tables(
     nat.require_cuda("build_paged_tables", context_lens, new_lens, block_tables, free_pages, num_free)
     dev, T = context_lens.device, int(num_tokens)
     ctx, new = context_lens.contiguous(), new_lens.contiguous()
-    out = PagedTables(torch.empty(T, dtype=torch.int64, device=dev), torch.empty(T, dtype=torch.int32, device=dev),
-                      torch.empty(T, dtype=torch.int32, device=dev), torch.empty(B + 1, dtype=torch.int32, device=dev),
-                      torch.empty(B, dtype=torch.int32, device=dev), torch.empty(1, dtype=torch.int32, device=dev))
+    slots = torch.empty(T, dtype=torch.int64, device=dev)
+    # the int32 results share one allocation, each on a 16-byte boundary
+    Tp, Bp = (T + 3) & ~3, (B + 4) & ~3
+    buf = torch.empty(2 * Tp + 2 * Bp + 4, dtype=torch.int32, device=dev)
+    rid, pos, cu, ctx_out, free_out = buf.as_strided((T,), (1,), 0), buf.as_strided((T,), (1,), Tp), \
+        buf.as_strided((B + 1,), (1,), 2 * Tp), buf.as_strided((B,), (1,), 2 * Tp + Bp), buf.as_strided((1,), (1,), 2 * Tp + 2 * Bp)
+    p0 = buf.data_ptr()
     nat.check(nat.lib().sa_paged_build_tables(
-        B, L, int(page_size), T, ctx.data_ptr(), new.data_ptr(), block_tables.data_ptr(), nat.strides(block_tables),
-        free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), int(position_base),
-        out.slot_mapping.data_ptr(), out.request_ids.data_ptr(), out.positions.data_ptr(), out.cu_new_lens.data_ptr(),
-        out.context_lens.data_ptr(), out.num_free.data_ptr(), nat.stream_of(ctx)), "build_paged_tables")
-    return out
+        B, L, int(page_size), T, ctx.data_ptr(), new.data_ptr(), block_tables.data_ptr(),
+        nat.cached_strides(block_tables), free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(),
+        int(position_base), slots.data_ptr(), p0, p0 + 4 * Tp, p0 + 8 * Tp, p0 + 4 * (2 * Tp + Bp),
+        p0 + 8 * (Tp + Bp), nat.raw_stream(ctx)), "build_paged_tables")
+    return PagedTables(slots, rid, pos, cu, ctx_out, free_out)
 
 
-@torch.no_grad()
 def release_paged_requests(
     finished: torch.Tensor,
     context_lens: torch.Tensor,
@@ -134,13 +136,12 @@ def release_paged_requests(
     ctx, done = context_lens.contiguous(), finished.contiguous()
     out_ctx, out_free = torch.empty_like(ctx), torch.empty(1, dtype=torch.int32, device=ctx.device)
     nat.check(nat.lib().sa_paged_release(
-        B, L, int(page_size), done.data_ptr(), ctx.data_ptr(), block_tables.data_ptr(), nat.strides(block_tables),
+        B, L, int(page_size), done.data_ptr(), ctx.data_ptr(), block_tables.data_ptr(), nat.cached_strides(block_tables),
         free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), out_ctx.data_ptr(), out_free.data_ptr(),
-        nat.stream_of(ctx)), "release_paged_requests")
+        nat.raw_stream(ctx)), "release_paged_requests")
     return out_ctx, out_free
 
 
-@torch.no_grad()
 def paged_kv_write(
     k: torch.Tensor,
     v: torch.Tensor,
@@ -167,7 +168,7 @@ def paged_kv_write(
                          f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
         raise ValueError("k, v, k_cache, v_cache must share dtype")
-    if slot_mapping.dtype != torch.int64 or tuple(slot_mapping.shape) != (T,):
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (T,):
         raise ValueError(f"slot_mapping must be int64 of shape {(T,)}, got {slot_mapping.dtype} "
                          f"{tuple(slot_mapping.shape)}")
     if (routes is None) != (router_indices is None):
@@ -186,10 +187,13 @@ def paged_kv_write(
     kk = k if k.stride(-1) == 1 else k.contiguous()
     vv = v if v.stride(-1) == 1 else v.contiguous()
     slots = slot_mapping.contiguous()
+    st = nat.cached_strides
+    if routes is None:
+        r_args = (None, 0, None, 0, 0, None, 0, None)
+    else:
+        r_args = (routes.data_ptr(), nat.int_code(routes.dtype), st(routes), H, TD, router_indices.data_ptr(),
+                  nat.int_code(router_indices.dtype), st(router_indices))
     nat.check(nat.lib().sa_paged_kv_write(
-        code, T, Hkv, D, k_cache.shape[2], k_cache.shape[0], kk.data_ptr(), nat.strides(kk), vv.data_ptr(),
-        nat.strides(vv), slots.data_ptr(), k_cache.data_ptr(), nat.strides(k_cache), v_cache.data_ptr(),
-        nat.strides(v_cache), nat.ptr(routes), nat.int_code(routes.dtype) if routes is not None else 0,
-        nat.strides(routes) if routes is not None else None, H, TD, nat.ptr(router_indices),
-        nat.int_code(router_indices.dtype) if routes is not None else 0,
-        nat.strides(router_indices) if routes is not None else None, nat.stream_of(k_cache)), "paged_kv_write")
+        code, T, Hkv, D, k_cache.shape[2], k_cache.shape[0], kk.data_ptr(), st(kk), vv.data_ptr(), st(vv),
+        slots.data_ptr(), k_cache.data_ptr(), st(k_cache), v_cache.data_ptr(), st(v_cache), *r_args,
+        nat.raw_stream(k_cache)), "paged_kv_write")

@@ -330,6 +330,24 @@ __global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const Pref
 // ---------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------
+// Bounded waits as in common.cuh, counted in tries instead of timed: half the instructions at each
+// of the kernel's dozen waits, which matters where every role's code competes for the
+// instruction cache.  A try on a phase that stays incomplete suspends the thread for about 8 k
+// cycles, so kMaxTries of them are about a second.
+constexpr uint32_t kMaxTries = 1u << 18;
+
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigned* st) {
+  for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n)
+    if (n == kMaxTries) {
+      raise_status(st, kStatusWaitTimeout);
+      return false;
+    }
+  return true;
+}
+__device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, unsigned* st) {
+  return __all_sync(0xffffffffu, wait_bar(bar, parity, st));
+}
+
 template <int DT, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_constant__ Args a) {
   using L = Layout<DT>;
@@ -511,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         uint4 m0, m1;
         while (more) {  // one descriptor per turn
           td = &descs[d % L::kDescs];
-          if (!(ok = mbar_wait_warp(&bars[L::bDEmpty + d % L::kDescs], ((d / L::kDescs) & 1) ^ 1, st))) break;
+          if (!(ok = wait_bar_warp(&bars[L::bDEmpty + d % L::kDescs], ((d / L::kDescs) & 1) ^ 1, st))) break;
           cur = 0;
           while (true) {
             if (done == total) {  // the next 32 entries
@@ -585,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       bool ok = true;
       while (ok) {
         const uint32_t ds = d % L::kDescs;
-        if (!mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+        if (!wait_bar_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
         const TileDesc& td = descs[ds];
         const int flags = td.flags;
         if (flags & F_END) break;
@@ -595,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
             const int tiles = flags & F_PAIR ? 2 : 1;
             for (int i = 0; i < tiles && ok; ++i, ++nq) {
               const uint32_t qb = nq & 1;
-              if (!(ok = mbar_wait_warp(&bars[L::bQEmpty + qb], ((nq >> 1) & 1) ^ 1, st))) break;
+              if (!(ok = wait_bar_warp(&bars[L::bQEmpty + qb], ((nq >> 1) & 1) ^ 1, st))) break;
               if (elect_one()) {
                 unsigned char* dst = sm + L::kQ + qb * L::kTile;
                 const uint32_t rows = (uint32_t)((flags & F_OWN) ? S.G : S.nb * S.G);
@@ -609,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           }
           for (int kv = 0; kv < 2 && ok; ++kv, ++seq) {
             const uint32_t sl = seq % L::kSlots;
-            if (!(ok = mbar_wait_warp(&bars[L::bEmpty + sl], ((seq / L::kSlots) & 1) ^ 1, st))) break;
+            if (!(ok = wait_bar_warp(&bars[L::bEmpty + sl], ((seq / L::kSlots) & 1) ^ 1, st))) break;
             if (elect_one()) {
               unsigned char* dst = sm + L::kRing + sl * L::kTile;
               mbar_arrive_expect_tx(&bars[L::bFull + sl], (uint32_t)(n * bn * 128 * dc));
@@ -715,26 +733,25 @@ int in_item = 0;          // key tiles of the item so far
         }
         const uint32_t pg = j0.bits & 1u, pph = (pg ? pc[1] : pc[0]) & 1;
         // nothing else to do before the older pending P arrives: wait for it
-        if (np == 2 && stage == 3 && !mbar_wait(&bars[L::bPFull + pg], pph, st)) break;
+        if (np == 2 && stage == 3 && !wait_bar(&bars[L::bPFull + pg], pph, st)) break;
         if (np > 0 && (np == 2 || stage != 3) && mbar_test(&bars[L::bPFull + pg], pph)) {
           // ---- O[g] += P V
           const uint32_t g = pg;
           const uint32_t seq = 2 * j0.tile + 1, sl = seq % L::kSlots;
           if (j0.bits & J_FIRST) {  // O[g] has been read by the last item's epilogue
-            if (!mbar_wait(&bars[L::bOFree + g], ((g ? of[1] : of[0]) & 1) ^ 1, st)) break;
+            if (!wait_bar(&bars[L::bOFree + g], ((g ? of[1] : of[0]) & 1) ^ 1, st)) break;
             if (g) ++of[1]; else ++of[0];
           }
-          if (!mbar_wait(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
+          if (!wait_bar(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
           const int n16 = (j0.vr + 15) & ~15;
           if (g) ++pc[1]; else ++pc[0];
           tc_fence_after();
-          const uint64_t vd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), kT * 128, 1024);
-          const uint32_t d_o = tmem + kColO + g * kT, a_p = tmem + kColS + g * kT;
-          const uint32_t acc = (j0.bits & J_FIRST) ? 0u : 1u;
-#pragma unroll
-          for (int kk = 0; kk < kT / 16; ++kk)
-            if (kk * 16 < n16)
-              tc_mma_f16_ts(d_o, a_p + kk * 8, desc_add(vd, kk * 16 * 128), id_pv, kk > 0 ? 1u : acc);
+          uint64_t vd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), kT * 128, 1024);
+          const uint32_t d_o = tmem + kColO + g * kT;
+          uint32_t a_p = tmem + kColS + g * kT, acc = (j0.bits & J_FIRST) ? 0u : 1u;
+#pragma unroll 1
+          for (int kk = 0; kk < n16; kk += 16, a_p += 8, acc = 1u, vd = desc_add(vd, 16 * 128))
+            tc_mma_f16_ts(d_o, a_p, vd, id_pv, acc);
           if (j0.bits & J_REL) tc_commit(&bars[L::bEmpty + sl]);
           if (j0.bits & J_LAST) tc_commit(&bars[L::bODone + g]);
           j0 = j1;
@@ -749,13 +766,15 @@ int in_item = 0;          // key tiles of the item so far
           const uint32_t g = job & 1, sl = (2 * tile) % L::kSlots, qb = (nq + rts - left) & 1;
           tc_fence_after();
           const uint32_t id_qk = idesc_f16(kT, (vr + 15) & ~15, BF16, false, false);
-          const uint64_t qd = smem_desc(smem_u32(sm + L::kQ + qb * L::kTile), 16, 1024);
-          const uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
+          uint64_t qd = smem_desc(smem_u32(sm + L::kQ + qb * L::kTile), 16, 1024);
+          uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
           const uint32_t d_s = tmem + kColS + g * kT;
-#pragma unroll
-          for (int kk = 0; kk < DT / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kT * 128) + (kk & 3) * 32;
-            if (kk < dk) tc_mma_f16(d_s, desc_add(qd, off), desc_add(kd, off), id_qk, kk > 0 ? 1u : 0u);
+#pragma unroll 1
+          for (int kk = 0; kk < dk; ++kk) {
+            tc_mma_f16(d_s, qd, kd, id_qk, kk > 0 ? 1u : 0u);
+            const uint32_t step = (kk & 3) == 3 ? kT * 128 - 96 : 32;  // the next 16 columns
+            qd = desc_add(qd, step);
+            kd = desc_add(kd, step);
           }
           tc_commit(&bars[L::bSFull + g]);
           if (left == 1) tc_commit(&bars[L::bEmpty + sl]);
@@ -808,7 +827,7 @@ int in_item = 0;          // key tiles of the item so far
     bool row_ok = false;
     while (true) {
       const uint32_t ds = d % L::kDescs;
-      if (!mbar_wait_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+      if (!wait_bar_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
       const TileDesc& td = descs[ds];
       const int flags = td.flags, vr = td.vr, slot = td.slot, n = td.n;
       if (flags & F_END) break;
@@ -838,7 +857,7 @@ int in_item = 0;          // key tiles of the item so far
         ++tile;
       }
       if (mine) {
-        if (!mbar_wait_warp(&bars[L::bSFull + grp], sc & 1, st)) break;
+        if (!wait_bar_warp(&bars[L::bSFull + grp], sc & 1, st)) break;
         ++sc;
         tc_fence_after();
         uint64_t ls = 0;
@@ -984,7 +1003,7 @@ int in_item = 0;          // key tiles of the item so far
           // V rows past the valid keys meet P = 0 in the product's last K step: they must be finite, so
           // they are cleared (in a pair tile by both groups, with the same zeros)
           const uint32_t seq = 2 * (tile - 1) + 1, sl = seq % L::kSlots;
-          if (!mbar_wait_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
+          if (!wait_bar_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
           unsigned char* vt = sm + L::kRing + sl * L::kTile;
           const int units = (16 - (vr & 15)) * (DT / 8);
 #pragma unroll 1
@@ -1010,7 +1029,7 @@ int in_item = 0;          // key tiles of the item so far
       float4* acc = (own ? a.w.acc_o : a.w.acc_p) + state * D4 * rows;
       if (row_ok) ml[rl] = make_float2(had ? m_used : -INFINITY, l_sum);
       if (had) {
-        if (!mbar_wait_warp(&bars[L::bODone + grp], od & 1, st)) break;
+        if (!wait_bar_warp(&bars[L::bODone + grp], od & 1, st)) break;
         ++od;
         tc_fence_after();
         if (__any_sync(0xffffffffu, row_ok)) {
@@ -1044,15 +1063,16 @@ int in_item = 0;          // key tiles of the item so far
 // ---------------------------------------------------------------------------------------
 // join of the partial states, one CTA per (request, KV head)
 // ---------------------------------------------------------------------------------------
-constexpr int kCombThreads = 512;  // at most
+constexpr int kCombThreads = 256;
 
 // Row (b, h) by itself, one warp: for rows whose joined state is not finite.  In the tensor-core
 // product a page's V meets every row of the tile, with weight 0 where the row does not attend
 // it; 0 * inf or 0 * NaN would leave a NaN in rows that have nothing to do with the page, so
-// such rows are computed again over their attended keys alone.  Costs tokens x ~100 cycles: only
+// such rows are computed again over their attended keys alone (columns d0..d1 of the output: those
+// of the calling CTA).  Costs tokens x ~100 cycles: only
 // non-finite values get here.
 template <typename T>
-__device__ __noinline__ void exact_row(const PrefixParams& p, int64_t b, int64_t h, float scale2) {
+__device__ __noinline__ void exact_row(const PrefixParams& p, int64_t b, int64_t h, float scale2, int d0, int d1) {
   const int lane = threadIdx.x & 31;
   const int64_t g = h / p.G, ptok = prefix_tokens(p), otok = own_tokens(p, b);
   const int64_t pp = (ptok + p.page - 1) / p.page, n = pp + (otok + p.page - 1) / p.page;
@@ -1085,36 +1105,33 @@ __device__ __noinline__ void exact_row(const PrefixParams& p, int64_t b, int64_t
   T* o = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < p.D) o[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] * (1.f / l));
-  if (p.lse && lane == 0) p.lse[b * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    if (lane + 32 * i >= d0 && lane + 32 * i < d1) o[lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : acc[i] * (1.f / l));
+  if (p.lse && lane == 0 && d0 == 0) p.lse[b * p.H + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
-// Thread = (head, float4 of the output); blockDim / cells groups of threads share a unit's states
-// where there are many of them and few units, and are joined through shared memory.  A chain of
-// three dependent round trips (plan, states, store): bound by latency, so all of a group's loads of
-// a round are issued together and nothing is divided here.
+// CTA = (unit, some of its cells); a cell is one head's float4 of the output.  CG groups of threads
+// share the states of the CTA's cells and are joined through shared memory.  A chain of three
+// dependent round trips (plan, states, store): bound by latency, so all of a group's loads of a round
+// are issued together and nothing is divided by more than CG here.
 template <typename T>
-__global__ void __launch_bounds__(kCombThreads, 2) prefix_combine_kernel(const __grid_constant__ PrefixParams p,
-                                                                         const Split s, const Ws w,
-                                                                         float scale2) {
+__global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const __grid_constant__ PrefixParams p,
+                                                                      const Split s, const Ws w, float scale2,
+                                                                      int cpb) {
   __shared__ float4 s_acc[kCombThreads];
   __shared__ float2 s_ml[kCombThreads];
   __shared__ unsigned s_bad[4];  // rows (of the group) to compute again
   const int G = s.G, D4 = s.D / 4, tid = threadIdx.x;
   const int b = blockIdx.x / s.Hkv, g = blockIdx.x - b * s.Hkv;
-  const int cells = G * D4;                       // float4 outputs of the unit
-  const int cpb = min(cells, (int)blockDim.x);    // cells per pass
-  const int CG = (int)blockDim.x / cpb;           // thread groups over the states
+  const int CG = kCombThreads / cpb;  // thread groups over the states
   const int cg = tid / cpb, ci = tid - cg * cpb;
   if (tid < 4) s_bad[tid] = 0;
   pdl_wait();
   const Pieces q = w.plan[blockIdx.x];
   const int total = q.n_p + q.n_o;
-#pragma unroll 1
-  for (int c0 = 0; c0 < cells; c0 += cpb) {
-    const int cell = c0 + ci;
-    const bool live = cg < CG && cell < cells;
-    const int c4 = live ? cell / G : 0, hh = live ? cell - c4 * G : 0;
+  const int cell0 = (int)blockIdx.y * cpb, cell = cell0 + ci, cells = G * D4;
+  const bool live = cell < cells;
+  const int c4 = live ? cell / G : 0, hh = live ? cell - c4 * G : 0;
+  {
     float M = -INFINITY, Ls = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     // (m, l) and acc of state (ml, x) into (M, Ls) and acc
@@ -1150,11 +1167,10 @@ __global__ void __launch_bounds__(kCombThreads, 2) prefix_combine_kernel(const _
       for (int u = 0; u < NU; ++u) fold(ml[u], x[u]);
     }
     if (CG > 1) {
-      __syncthreads();  // the last pass's shared states are read
       s_acc[tid] = acc;
       s_ml[tid] = make_float2(M, Ls);
-      __syncthreads();
     }
+    __syncthreads();
     if (cg == 0 && live) {
 #pragma unroll 1
       for (int c = 1; c < CG; ++c) fold(s_ml[c * cpb + ci], s_acc[c * cpb + ci]);
@@ -1171,8 +1187,11 @@ __global__ void __launch_bounds__(kCombThreads, 2) prefix_combine_kernel(const _
     }
   }
   __syncthreads();
-  for (int hh = tid >> 5; hh < G; hh += (int)blockDim.x / 32)
-    if ((s_bad[hh >> 5] >> (hh & 31)) & 1u) exact_row<T>(p, b, g * G + hh, scale2);
+  // (the CTA's cells of head r are the columns 4 c with cell0 <= c G + r < cell0 + cpb)
+  for (int r = tid >> 5; r < G; r += kCombThreads / 32)
+    if ((s_bad[r >> 5] >> (r & 31)) & 1u)
+      exact_row<T>(p, b, g * G + r, scale2, 4 * max(0, (cell0 - r + G - 1) / G),
+                   4 * min(D4, max(0, (cell0 + cpb - r + G - 1) / G)));
 }
 
 template <int DT, bool BF16>
@@ -1268,18 +1287,18 @@ int launch_prefix_fast(const PrefixParams& p, int dtype, void* workspace, cudaSt
   else
     rc = bf ? launch_main<128, true>(a, a.masked, stream) : launch_main<128, false>(a, a.masked, stream);
   if (rc) return rc;
-  // Threads per unit: one group of threads per unit where the units fill the GPU by themselves, up
-  // to 8 where they do not (a unit then has many states: with few units the prefix is cut finely).
-  const int cells = (int)(p.G * p.D / 4);
-  const int64_t units = p.B * p.Hkv;
-  const int groups = units >= 1024 ? 1 : units >= 512 ? 2 : units >= 256 ? 4 : 8;
-  const int threads = std::min(kCombThreads, (std::min(cells, kCombThreads) * groups + 31) / 32 * 32);
-  const dim3 grid((unsigned)units), block((unsigned)threads);
+  // Groups of threads per cell: enough to fill the GPU with threads, 16 at most; a batch with few
+  // cells is one whose prefix is cut finely, with many states to join.
+  const int64_t cells = p.G * p.D / 4, all = cells * p.B * p.Hkv, fill = (int64_t)device_sm_count() * 1024;
+  int groups = 1;
+  while (groups < 16 && all * groups * 2 <= fill) groups *= 2;
+  const int cpb = kCombThreads / groups;
+  const dim3 grid((unsigned)(p.B * p.Hkv), (unsigned)((cells + cpb - 1) / cpb)), block(kCombThreads);
   if (bf)
     return launch_dependent(prefix_combine_kernel<__nv_bfloat16>, grid, block, 0, stream, "prefix_combine_kernel", p, a.s,
-                            a.w, a.scale2);
+                            a.w, a.scale2, cpb);
   return launch_dependent(prefix_combine_kernel<__half>, grid, block, 0, stream, "prefix_combine_kernel", p, a.s, a.w,
-                          a.scale2);
+                          a.scale2, cpb);
 }
 
 }  // namespace sa

@@ -50,9 +50,11 @@ constexpr uint32_t kMaxSmem = 232448;
 constexpr float kRescaleThreshold = 8.0f;   // log2 units
 constexpr int kMaxHeadWords = 8;            // query heads <= 256 (mask kernel)
 
-// Weights of one key tile in the split of the work over CTAs: a pair tile keeps the tensor and
-// exponential pipes busy about one and a half times as long as any tile's load takes.
-constexpr int kWPair = 3, kWOne = 2;
+// Cost of one key tile in the split of the work over CTAs, in units of about 250 cycles (traced): a
+// pair tile, a tile of either other kind, and what an item costs besides its tiles (fill, drain and
+// partial states; of a pair item twice that), spread over its tiles.  With routing, own and single
+// tiles count by the share of their pages that some row attends.
+constexpr int kCostPair = 16, kCostOne = 11, kCostItem = 14;
 
 enum { F_FIRST = 1, F_LAST = 2, F_EMPTY = 4, F_END = 8, F_PAIR = 16, F_OWN = 32 };
 
@@ -118,6 +120,8 @@ struct Ws {
   float4* acc_p;      // [prefix slots][2][D / 4][128]
   float2* ml_o;       // [own slots][2][G]
   float4* acc_o;      // [own slots][2][D / 4][G]
+  int* cnt_o;         // [B][chunks of own pages] selected (page, KV head) pairs
+  int* cnt_p;         // [Hkv][chunks of prefix pages] pages attended by the last row tile's first 32 rows
   int WO;
 };
 
@@ -157,6 +161,11 @@ inline Split make_split(int64_t B, int64_t G, int64_t Hkv, int64_t page, int64_t
   return s;
 }
 
+// Chunks of kMaskPages pages (the mask kernel's tasks).
+constexpr int kMaskPages = 16;
+__host__ __device__ inline int prefix_chunks(const Split& s) { return (s.Lp + kMaskPages - 1) / kMaskPages; }
+__host__ __device__ inline int own_chunks(const Split& s) { return (s.L + kMaskPages - 1) / kMaskPages; }
+
 inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 size_t carve(void* base, const Split& s, Ws* w) {
@@ -174,6 +183,8 @@ size_t carve(void* base, const Split& s, Ws* w) {
   t.plan = reinterpret_cast<Pieces*>(take((size_t)B * Hkv * sizeof(Pieces)));
   t.mask_p = reinterpret_cast<uint32_t*>(take((size_t)Hkv * s.row_tiles * Lp * 16));
   t.mask_o = reinterpret_cast<uint32_t*>(take((size_t)B * Hkv * L * t.WO * 4));
+  t.cnt_o = reinterpret_cast<int*>(take((size_t)B * own_chunks(s) * 4));
+  t.cnt_p = reinterpret_cast<int*>(take((size_t)Hkv * prefix_chunks(s) * 4));
   t.ml_p = reinterpret_cast<float2*>(take(sp * 2 * kT * 8));
   t.acc_p = reinterpret_cast<float4*>(take(sp * 2 * kT * D * 4));
   t.ml_o = reinterpret_cast<float2*>(take(so * 2 * G * 8));
@@ -187,6 +198,7 @@ size_t carve(void* base, const Split& s, Ws* w) {
 // ---------------------------------------------------------------------------------------
 struct Line {
   int tiles_p;      // key tiles of the prefix
+  int wt[3];        // weight of a tile of each segment
   int64_t len[3];   // weighted lengths of the segments
   int64_t W;
   int n;            // CTAs that get a range
@@ -202,16 +214,38 @@ __device__ __forceinline__ int tiles_of(const Split& s, int n) {
   return (int)(((unsigned)n + (unsigned)s.span - 1u) / (unsigned)s.span) * s.sub;
 }
 
-__device__ __forceinline__ Line make_line(const Split& s, int prefix_tokens, int own_total) {
+// own_pages: selected (page, KV head) pairs of the own part; seen: selected (page, KV head) pairs
+// of the single segment's first 32 rows.  Negative: all.
+__device__ __forceinline__ Line make_line(const Split& s, int prefix_tokens, int own_total, int own_pages, int seen) {
   Line l;
   l.tiles_p = tiles_of(s, prefix_tokens);
-  l.len[0] = (int64_t)s.units[0] * l.tiles_p * kWPair;
-  l.len[1] = (int64_t)s.units[1] * l.tiles_p * kWOne;
-  l.len[2] = (int64_t)own_total * s.Hkv * kWOne;
+  const int tiles1 = max(1, l.tiles_p);
+  l.wt[0] = kCostPair + 2 * kCostItem / tiles1;
+  l.wt[1] = kCostOne + kCostItem / tiles1;
+  l.wt[2] = kCostOne;
+  const int pages = (prefix_tokens + s.page - 1) / s.page;
+  if (seen >= 0 && s.units[1] > 0 && pages > 0) {
+    // pages that none of the row tile's 32-row words attends, taken as independent
+    const int words = ((s.B - (s.row_tiles - 1) * s.nb) * s.G + 31) / 32;
+    const float none = 1.f - (float)seen / ((float)s.Hkv * (float)pages);
+    float all = none;
+#pragma unroll 1
+    for (int w = 1; w < words; ++w) all *= none;
+    l.wt[1] = max(1, (int)(kCostOne * (1.f - all) + 0.5f) + kCostItem / tiles1);
+  }
+  if (own_total > 0) {
+    const float tiles = (float)own_total * (float)s.Hkv;
+    const float full = own_pages < 0 ? tiles : (float)own_pages / (float)s.ppt * (float)s.sub;
+    const float items = (float)min(s.B, own_total) * (float)s.Hkv;
+    l.wt[2] = max(1, (int)((kCostOne * min(full, tiles) + kCostItem * items) / tiles + 0.5f));
+  }
+  l.len[0] = (int64_t)s.units[0] * l.tiles_p * l.wt[0];
+  l.len[1] = (int64_t)s.units[1] * l.tiles_p * l.wt[1];
+  l.len[2] = (int64_t)own_total * s.Hkv * l.wt[2];
   l.W = l.len[0] + l.len[1] + l.len[2];
   // every range spans at least one tile of the heaviest kind, so that a CTA whose range lies inside
   // a unit holds a piece of it
-  l.n = (int)max((int64_t)1, min((int64_t)s.grid, l.W / kWPair));
+  l.n = (int)max((int64_t)1, min((int64_t)s.grid, l.W / max(l.wt[0], max(l.wt[1], l.wt[2]))));
   return l;
 }
 
@@ -234,7 +268,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
 // Warp task: 16 pages against 32 rows (prefix: rows of one mask word; own: 32 heads at a time of one
 // request).  Lane = row: its r levels against the 16 pages' vectors, 16 loads in flight per
 // level; a ballot per page is the page's mask word.  Integer compares of a few MB that sit in L2.
-constexpr int kMaskPages = 16;
 constexpr int kMaskWarps = 4;
 
 template <typename RT>
@@ -271,7 +304,11 @@ __global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const Pref
       const int word = (int)(x % 4);
       x /= 4;
       const int64_t rt = x % s.row_tiles, g = x / s.row_tiles;
-      if (l0 >= pre_pages) continue;
+      const bool counted = word == 0 && rt == s.row_tiles - 1 && (s.row_tiles & 1);
+      if (l0 >= pre_pages) {
+        if (counted && lane == 0) w.cnt_p[g * chunks + l0 / kMaskPages] = 0;
+        continue;
+      }
       const int row = word * 32 + lane;
       const int64_t b = rt * s.nb + row / p.G, h = g * p.G + row % p.G;
       const bool live = row < s.nb * p.G && b < p.B;
@@ -279,18 +316,27 @@ __global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const Pref
       if (phys < 0 || phys >= p.num_pages) phys = 0;  // dropped by the scheduler
       uint32_t bits = match(phys, live ? b : 0, live ? h : 0);
       const int64_t n = pre_pages + (live ? (own_tokens(p, b) + p.page - 1) / p.page : 0);
+      int count = 0;
       for (int u = 0; u < kMaskPages; ++u) {
         const int64_t l = l0 + u;
         const bool on = ((bits >> u) & 1u) || (p.sink && l == 0) || l >= n - p.local_blocks;
         const uint32_t m = __ballot_sync(0xffffffffu, live && on);
-        if (lane == 0 && l < pre_pages) w.mask_p[((g * s.row_tiles + rt) * p.Lp + l) * 4 + word] = m;
+        if (l < pre_pages) {
+          count += m != 0u;
+          if (lane == 0) w.mask_p[((g * s.row_tiles + rt) * p.Lp + l) * 4 + word] = m;
+        }
       }
+      if (counted && lane == 0) w.cnt_p[g * chunks + l0 / kMaskPages] = count;
     } else {
       int64_t x = task - prefix_tasks;
       const int64_t chunks = (p.L + kMaskPages - 1) / kMaskPages;
       const int64_t l0 = (x % chunks) * kMaskPages, b = x / chunks;
       const int64_t pages = (own_tokens(p, b) + p.page - 1) / p.page;
-      if (l0 >= pages) continue;
+      if (l0 >= pages) {
+        if (lane == 0) w.cnt_o[task - prefix_tasks] = 0;
+        continue;
+      }
+      int count = 0;  // (page, KV head) pairs that some head attends
       int phys = lane < kMaskPages && l0 + lane < pages ? p.bt[b * p.bts[0] + (l0 + lane) * p.bts[1]] : 0;
       if (phys < 0 || phys >= p.num_pages) phys = 0;
       const int HW = (int)((p.H + 31) / 32);
@@ -321,7 +367,11 @@ __global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const Pref
           if (cnt < 32) m &= (1u << cnt) - 1u;
         }
         w.mask_o[((b * p.Hkv + g) * p.L + l0 + u) * w.WO + wd] = m;
+        count += m != 0u;
       }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+      if (lane == 0) w.cnt_o[task - prefix_tasks] = count;
       __syncwarp();
     }
   }
@@ -367,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
   TileDesc* descs = reinterpret_cast<TileDesc*>(sm + L::kDesc);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + L::kMisc);
   int* s_warp = reinterpret_cast<int*>(sm + L::kMisc + 16);       // [12] scan
-  int* s_start = reinterpret_cast<int*>(sm + L::kMisc + 80);      // first own request, tiles before it
+  int* s_start = reinterpret_cast<int*>(sm + L::kMisc + 64);      // first own request, tiles before it
+  int* s_cnt = reinterpret_cast<int*>(sm + L::kMisc + 80);        // [12][2] selected pages
   const Split& S = a.s;
   unsigned* st = a.status;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -414,6 +465,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
   if (lane == 31) s_warp[warp] = incl;
   if (threadIdx.x == 0) s_start[0] = S.B;
   const int ptok = pre_tokens(S, a.plen_dev, a.plen);
+  if (a.masked) {  // selected pages, for the tiles' weights
+    pdl_wait();    // the row masks and their counts are complete from here on
+    int2 sel = make_int2(0, 0);
+    const int no = S.B * own_chunks(S), npc = S.units[1] > 0 ? S.Hkv * prefix_chunks(S) : 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < no; i += kThreads) sel.x += __ldcg(a.w.cnt_o + i);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < npc; i += kThreads) sel.y += __ldcg(a.w.cnt_p + i);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      sel.x += __shfl_xor_sync(0xffffffffu, sel.x, o);
+      sel.y += __shfl_xor_sync(0xffffffffu, sel.y, o);
+    }
+    if (lane == 0) {
+      s_cnt[2 * warp] = sel.x;
+      s_cnt[2 * warp + 1] = sel.y;
+    }
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -424,7 +493,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     before += w < warp ? t : 0;
     own_total += t;
   }
-  const Line line = make_line(S, ptok, own_total);
+  int own_pages = -1, seen = -1;
+  if (a.masked) {
+    own_pages = seen = 0;
+#pragma unroll 1
+    for (int w = 0; w < kThreads / 32; ++w) {
+      own_pages += s_cnt[2 * w];
+      seen += s_cnt[2 * w + 1];
+    }
+  }
+  const Line line = make_line(S, ptok, own_total, own_pages, seen);
   const bool active = (int)blockIdx.x < line.n && line.W > 0;
   const int64_t x0 = active ? range_start(line, blockIdx.x) : 0, x1 = active ? range_start(line, blockIdx.x + 1) : 0;
   // the CTA's tiles [lo, hi) of a segment that starts at `base` and whose tiles weigh wt
@@ -434,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
   };
   const int64_t own_base = line.len[0] + line.len[1];
   // own tiles [k0, k1) of the CTA; the thread whose requests hold k0 publishes the first one
-  const int k0 = seg_lo(own_base, kWOne), k1 = seg_hi(own_base, line.len[2], kWOne);
+  const int k0 = seg_lo(own_base, line.wt[2]), k1 = seg_hi(own_base, line.len[2], line.wt[2]);
   {
     int c = before;
 #pragma unroll 1
@@ -455,7 +533,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
     if (warp == kSchedWarp) {
       // ---------------------------------------------------------------- scheduler
-      if (a.masked) pdl_wait();  // the row masks
       const int ppt = S.ppt, sub = S.sub, bn = S.bn;
       uint32_t d = 0;  // descriptors pushed
       bool ok = true;
@@ -478,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
             }
           } else {
             const int64_t base = seg ? line.len[0] : 0, len = seg ? line.len[1] : line.len[0];
-            const int wt = seg ? kWOne : kWPair;
+            const int wt = seg ? line.wt[1] : line.wt[0];
             k = seg_lo(base, wt);
             hi = seg_hi(base, len, wt);
           }
@@ -666,16 +743,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         for (int g = lane; g < S.Hkv; g += 32) {
           Pieces q{0, 0, pr ? 2 : 1, (b - rt * S.nb) * S.G, 0, 0, {0, 0}};
           if (line.tiles_p > 0) {
-            const int u = pr ? g * pairs + rt / 2 : S.units[0] + g, wt = pr ? kWPair : kWOne;
-            const int64_t x = pr ? (int64_t)u * line.tiles_p * kWPair : line.len[0] + (int64_t)g * line.tiles_p * kWOne;
+            const int u = pr ? g * pairs + rt / 2 : S.units[0] + g, wt = pr ? line.wt[0] : line.wt[1];
+            const int64_t x = pr ? (int64_t)u * line.tiles_p * wt : line.len[0] + (int64_t)g * line.tiles_p * wt;
             const int i0 = range_of(line, x);
             q.n_p = (range_of(line, x + (int64_t)(line.tiles_p - 1) * wt) - i0 + 1) * (pr ? 1 : 2);
             q.first_p = (u + i0) * 2 + (pr ? rt & 1 : 0);
           }
           if (t > 0) {
-            const int64_t x = own_base + ((int64_t)cum * S.Hkv + g * t) * kWOne;
+            const int64_t x = own_base + ((int64_t)cum * S.Hkv + g * t) * line.wt[2];
             const int i0 = range_of(line, x);
-            q.n_o = (range_of(line, x + (int64_t)(t - 1) * kWOne) - i0 + 1) * 2;
+            q.n_o = (range_of(line, x + (int64_t)(t - 1) * line.wt[2]) - i0 + 1) * 2;
             q.first_o = (b * S.Hkv + g + i0) * 2;
           }
           a.w.plan[(int64_t)b * S.Hkv + g] = q;
@@ -1235,8 +1312,8 @@ bool prefix_fast_eligible(const PrefixParams& p, int dtype) {
   if (p.num_pages < 1 || p.num_pages > INT32_MAX) return false;
   // weighted key tiles of the whole batch stay below 2^31
   const int64_t span = std::max<int64_t>(8, std::min<int64_t>(p.page, kT));
-  if ((double)p.B * p.Hkv * (p.L + 1) * (p.page / span + 1) * kWPair > 1e9 ||
-      (double)p.B * p.Hkv * (p.Lp + 1) * (p.page / span + 1) * kWPair > 1e9)
+  if ((double)p.B * p.Hkv * (p.L + 1) * (p.page / span + 1) * 32 > 1e9 ||
+      (double)p.B * p.Hkv * (p.Lp + 1) * (p.page / span + 1) * 32 > 1e9)
     return false;
   if (reinterpret_cast<uintptr_t>(p.q) % 16 || reinterpret_cast<uintptr_t>(p.kc) % 16 ||
       reinterpret_cast<uintptr_t>(p.vc) % 16)

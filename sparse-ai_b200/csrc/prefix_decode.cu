@@ -14,7 +14,8 @@
 // This file: the entry point and the general path (any head_dim up to 256, any page size,
 // stride and element type; fp32 arithmetic on the CUDA cores).  A CTA takes up to kRows rows of one
 // KV head and a range of 32-key tiles: K and V of a tile go to shared memory once and serve all
-// its rows.  It is bound by its shared-memory reads (5 words for 4 products).
+// its rows, as float4s: 16 products per 5 loads.  Batches that need it are small (a 32-bit cache, odd
+// sizes), so it is bound by latency along its few tiles.
 #include <algorithm>
 #include <string>
 
@@ -35,8 +36,8 @@ struct PdSplit {
   int sp, so;                // splits of the prefix's and of each request's own keys
 };
 
-// Splits so that both kinds of work reach about four CTAs per SM, with at least two key tiles
-// each over the lists' widths (the lengths are on the device).
+// Splits so that both kinds of work reach about four CTAs per SM, down to one key tile each over the
+// lists' widths (the lengths are on the device): a tile takes a CTA about 10 us, all latency.
 PdSplit pd_split(int64_t B, int64_t H, int64_t Hkv, int64_t page, int64_t Lp, int64_t L) {
   PdSplit s;
   const int64_t G = H / Hkv;
@@ -44,7 +45,7 @@ PdSplit pd_split(int64_t B, int64_t H, int64_t Hkv, int64_t page, int64_t Lp, in
   s.own_tiles = (int)((G + kRows - 1) / kRows);
   auto splits = [](int64_t ctas, int64_t tokens) {
     const int64_t want = (4 * 148 + ctas - 1) / std::max<int64_t>(ctas, 1);
-    const int64_t cap = (tokens + 2 * kKeys - 1) / (2 * kKeys);
+    const int64_t cap = (tokens + kKeys - 1) / kKeys;
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, cap, kMaxSplits}));
   };
   s.sp = Lp > 0 ? splits(Hkv * s.row_tiles, Lp * page) : 0;
@@ -57,15 +58,20 @@ int64_t pd_bytes(int64_t B, int64_t H, int64_t D, const PdSplit& s) {
   return B * H * (int64_t)(s.sp + s.so) * (D + 2) * 4;
 }
 
-template <typename T>
+// NI: float4 output columns per thread, D <= 32 NI.
+template <typename T, int NI>
 __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixParams p, const PdSplit s, float* part) {
   extern __shared__ float sm[];
-  const int D = (int)p.D, DP = D + 1;
-  float* s_q = sm;                    // [kRows][D + 1]
-  float* s_k = s_q + kRows * DP;      // [kKeys][D + 1]
-  float* s_v = s_k + kKeys * DP;      // [kKeys][D + 1]
+  // rows of D floats, padded with zeros to whole float4s and by one more, so that the eight keys that
+  // a row's threads read at a time lie in different banks
+  const int D = (int)p.D, D4 = (D + 3) / 4, DP = 4 * D4 + 4;
+  float* s_q = sm;                    // [kRows][DP]
+  float* s_k = s_q + kRows * DP;      // [kKeys][DP]
+  float* s_v = s_k + kKeys * DP;      // [kKeys][DP]
   float* s_p = s_v + kKeys * DP;      // [kRows][kKeys + 1]
-  __shared__ int64_t s_phys[kKeys];   // page of each key of the tile (-1: none)
+  // page of each key of the tile (-1: none), its logical index, and the key's K and V rows
+  __shared__ int s_phys[kKeys], s_lp[kKeys];
+  __shared__ const T *s_krow[kKeys], *s_vrow[kKeys];
   const int tid = threadIdx.x;
 
   // ---- which rows and which keys
@@ -105,45 +111,48 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
   const int64_t b = live ? (row0 + row) / p.G : 0, h = live ? g * p.G + (row0 + row) % p.G : 0;
   const int64_t n_pages = pre_pages + (live ? (own_tokens(p, b) + p.page - 1) / p.page : 0);
   const float scale2 = rsqrtf((float)D) * kLog2e;
-  for (int i = tid; i < kRows * D; i += kPdThreads) {
-    const int rr = i / D, d = i - rr * D;
-    float v = 0.f;
-    if (rr < nrows) {
-      const int64_t bb = (row0 + rr) / p.G, hh = g * p.G + (row0 + rr) % p.G;
-      v = to_f32<T>(static_cast<const T*>(p.q)[bb * p.qs[0] + hh * p.qs[1] + d]) * scale2;
+  {
+    const int warp = tid >> 5, lane = tid & 31;
+    for (int rr = warp; rr < kRows; rr += kPdThreads / 32) {
+      const int rg = (int)row0 + rr, bb = rg / (int)p.G, hh = (int)g * (int)p.G + rg - bb * (int)p.G;
+      const T* q = static_cast<const T*>(p.q) + bb * p.qs[0] + hh * p.qs[1];
+      for (int d = lane; d < 4 * D4; d += 32) s_q[rr * DP + d] = rr < nrows && d < D ? to_f32<T>(q[d]) * scale2 : 0.f;
     }
-    s_q[rr * DP + d] = v;
   }
-  float m = -INFINITY, l = 0.f, acc[kMaxD / kTpr];
+  float m = -INFINITY, l = 0.f;
+  float4 acc[NI];
 #pragma unroll
-  for (int i = 0; i < kMaxD / kTpr; ++i) acc[i] = 0.f;
+  for (int i = 0; i < NI; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
 
   for (int64_t t = t_lo; t < t_hi; ++t) {
     __syncthreads();  // the last tile's shared arrays are read
     if (tid < kKeys) {
-      const int64_t tok = t * kKeys + tid;
-      int64_t phys = -1;
+      const int tok = (int)(t * kKeys) + tid;
+      int phys = -1, lp = 0;
       if (tok < tokens) {
-        const int64_t lp = tok / p.page;
+        lp = tok / (int)p.page;
         phys = own ? p.bt[b_own * p.bts[0] + lp * p.bts[1]] : p.ppages[lp];
         if (phys < 0 || phys >= p.num_pages) {
           raise_status(p.status, kStatusBadIndex);
           phys = -1;
         }
+        const int off = tok - lp * (int)p.page;
+        s_krow[tid] = static_cast<const T*>(p.kc) + (int64_t)phys * p.ks[0] + g * p.ks[1] + off * p.ks[2];
+        s_vrow[tid] = static_cast<const T*>(p.vc) + (int64_t)phys * p.vs[0] + g * p.vs[1] + off * p.vs[2];
       }
       s_phys[tid] = phys;
+      s_lp[tid] = lp;
     }
     __syncthreads();
     // keys of this row in the tile: li, li + kTpr, ...
     bool see[kKeys / kTpr], any = false;
-    int64_t last_lp = -1;
+    int last_lp = -1;
     bool last_on = false;
 #pragma unroll
     for (int u = 0; u < kKeys / kTpr; ++u) {
-      const int64_t tok = t * kKeys + li + u * kTpr, phys = s_phys[li + u * kTpr];
+      const int phys = s_phys[li + u * kTpr], lp = s_lp[li + u * kTpr];
       see[u] = live && phys >= 0;
-      if (see[u]) {
-        const int64_t lp = tok / p.page;
+      if (see[u] && p.r > 0) {
         if (lp != last_lp) {
           last_lp = lp;
           last_on = page_attended(p, b, h, (own ? pre_pages : 0) + lp, n_pages, phys);
@@ -153,25 +162,29 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
       any |= see[u];
     }
     if (!__syncthreads_or(any)) continue;
-    for (int i = tid; i < kKeys * D; i += kPdThreads) {
-      const int kk = i / D, d = i - kk * D;
-      const int64_t phys = s_phys[kk], off = (t * kKeys + kk) % p.page;
-      float kv = 0.f, vv = 0.f;
-      if (phys >= 0) {
-        kv = to_f32<T>(static_cast<const T*>(p.kc)[phys * p.ks[0] + g * p.ks[1] + off * p.ks[2] + d]);
-        vv = to_f32<T>(static_cast<const T*>(p.vc)[phys * p.vs[0] + g * p.vs[1] + off * p.vs[2] + d]);
+    // one warp per key, lanes along the row; all of a warp's loads in flight
+    const int warp = tid >> 5, lane = tid & 31;
+    for (int d = lane; d < 4 * D4; d += 32) {
+#pragma unroll
+      for (int u = 0; u < kKeys / (kPdThreads / 32); ++u) {
+        const int kk = warp + u * (kPdThreads / 32);
+        const bool have = s_phys[kk] >= 0 && d < D;
+        s_k[kk * DP + d] = have ? to_f32<T>(s_krow[kk][d]) : 0.f;
+        s_v[kk * DP + d] = have ? to_f32<T>(s_vrow[kk][d]) : 0.f;
       }
-      s_k[kk * DP + d] = kv;
-      s_v[kk * DP + d] = vv;
     }
     __syncthreads();
     float sc[kKeys / kTpr];
 #pragma unroll
     for (int u = 0; u < kKeys / kTpr; ++u) sc[u] = 0.f;
-    for (int d = 0; d < D; ++d) {
-      const float qd = s_q[row * DP + d];
+#pragma unroll 4
+    for (int d = 0; d < D4; ++d) {
+      const float4 q = *reinterpret_cast<const float4*>(s_q + row * DP + 4 * d);
 #pragma unroll
-      for (int u = 0; u < kKeys / kTpr; ++u) sc[u] = fmaf(qd, s_k[(li + u * kTpr) * DP + d], sc[u]);
+      for (int u = 0; u < kKeys / kTpr; ++u) {
+        const float4 k = *reinterpret_cast<const float4*>(s_k + (li + u * kTpr) * DP + 4 * d);
+        sc[u] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, sc[u]))));
+      }
     }
     float mt = -INFINITY;
 #pragma unroll
@@ -195,14 +208,26 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
     l = l * alpha + ps;
     m = m_new;
 #pragma unroll
-    for (int i = 0; i < kMaxD / kTpr; ++i) acc[i] *= alpha;
+    for (int i = 0; i < NI; ++i) {
+      acc[i].x *= alpha;
+      acc[i].y *= alpha;
+      acc[i].z *= alpha;
+      acc[i].w *= alpha;
+    }
     __syncwarp();  // a row's threads are one warp's
+#pragma unroll 4
     for (int kk = 0; kk < kKeys; ++kk) {
       const float e = s_p[row * (kKeys + 1) + kk];
-      if (e < 0.f) continue;  // masked: whatever V holds there does not count
+      const bool on = !(e < 0.f);  // masked: whatever V holds there does not count
 #pragma unroll
-      for (int i = 0; i < kMaxD / kTpr; ++i)
-        if (li + i * kTpr < D) acc[i] = fmaf(e, s_v[kk * DP + li + i * kTpr], acc[i]);
+      for (int i = 0; i < NI; ++i)
+        if (li + i * kTpr < D4) {
+          const float4 v = *reinterpret_cast<const float4*>(s_v + kk * DP + 4 * (li + i * kTpr));
+          acc[i].x = on ? fmaf(e, v.x, acc[i].x) : acc[i].x;
+          acc[i].y = on ? fmaf(e, v.y, acc[i].y) : acc[i].y;
+          acc[i].z = on ? fmaf(e, v.z, acc[i].z) : acc[i].z;
+          acc[i].w = on ? fmaf(e, v.w, acc[i].w) : acc[i].w;
+        }
     }
   }
   if (!live) return;
@@ -212,8 +237,13 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
     o[1] = l;
   }
 #pragma unroll
-  for (int i = 0; i < kMaxD / kTpr; ++i)
-    if (li + i * kTpr < D) o[2 + li + i * kTpr] = acc[i];
+  for (int i = 0; i < NI; ++i) {
+    const int c = 4 * (li + i * kTpr);
+    if (c < D) o[2 + c] = acc[i].x;
+    if (c + 1 < D) o[3 + c] = acc[i].y;
+    if (c + 2 < D) o[4 + c] = acc[i].z;
+    if (c + 3 < D) o[5 + c] = acc[i].w;
+  }
 }
 
 // Joins the parts of (b, h) = blockIdx.x.
@@ -221,25 +251,37 @@ template <typename T>
 __global__ void __launch_bounds__(kPdThreads) prefix_join_kernel(const PrefixParams p, const PdSplit s,
                                                                  const float* part) {
   const int64_t b = blockIdx.x / p.H, h = blockIdx.x % p.H;
-  const int n = s.sp + s.so, D = (int)p.D;
+  const int n = s.sp + s.so, D = (int)p.D, tid = threadIdx.x;
   const float* base = part + (int64_t)blockIdx.x * n * (D + 2);
+  __shared__ float s_m[2 * kMaxSplits], s_w[2 * kMaxSplits];
+  __shared__ float s_l[2 * kMaxSplits];
+  if (tid < n) {  // n <= 2 kMaxSplits == kPdThreads
+    s_m[tid] = base[(int64_t)tid * (D + 2)];
+    s_l[tid] = base[(int64_t)tid * (D + 2) + 1];
+  }
+  __syncthreads();
   float M = -INFINITY;
-  for (int i = 0; i < n; ++i) M = fmaxf(M, base[(int64_t)i * (D + 2)]);
+  for (int i = 0; i < n; ++i) M = fmaxf(M, s_m[i]);
   const float ref = M == -INFINITY ? 0.f : M;
+  if (tid < n) s_w[tid] = exp2f(s_m[tid] - ref);
+  __syncthreads();
   float L = 0.f;
-  for (int i = 0; i < n; ++i) L += base[(int64_t)i * (D + 2) + 1] * exp2f(base[(int64_t)i * (D + 2)] - ref);
+  for (int i = 0; i < n; ++i) L += s_l[i] * s_w[i];
   const float inv = L == 0.f ? 0.f : 1.f / L;  // NaN stays NaN
   T* o = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1];
-  for (int d = threadIdx.x; d < D; d += kPdThreads) {
+  for (int d = tid; d < D; d += kPdThreads) {
     float a = 0.f;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) {
-      const float* e = base + (int64_t)i * (D + 2);
-      if (e[0] != -INFINITY) a += e[2 + d] * exp2f(e[0] - ref);
+      const float x = base[(int64_t)i * (D + 2) + 2 + d];
+      if (s_m[i] != -INFINITY) a = fmaf(x, s_w[i], a);
     }
     o[d] = from_f32<T>(L == 0.f ? 0.f : a * inv);
   }
-  if (p.lse && threadIdx.x == 0) p.lse[blockIdx.x] = L == 0.f ? -INFINITY : M * kLn2 + logf(L);
+  if (p.lse && tid == 0) p.lse[blockIdx.x] = L == 0.f ? -INFINITY : M * kLn2 + logf(L);
 }
+
+static_assert(2 * kMaxSplits == kPdThreads, "one thread per part in the join");
 
 template <typename T>
 int launch_general(const PrefixParams& p, float* part, cudaStream_t stream) {
@@ -247,9 +289,12 @@ int launch_general(const PrefixParams& p, float* part, cudaStream_t stream) {
   const int64_t ctas = p.Hkv * s.row_tiles * s.sp + p.B * p.Hkv * s.own_tiles * s.so;
   if (ctas > INT32_MAX) return fail(SA_EUNSUPPORTED, "prefix decode: too many requests");
   if (ctas > 0) {
-    const size_t smem = ((size_t)(kRows + 2 * kKeys) * (p.D + 1) + kRows * (kKeys + 1)) * 4;
-    cudaFuncSetAttribute(prefix_split_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    prefix_split_kernel<T><<<(unsigned)ctas, kPdThreads, smem, stream>>>(p, s, part);
+    const size_t smem = ((size_t)(kRows + 2 * kKeys) * ((p.D + 3) / 4 * 4 + 4) + kRows * (kKeys + 1)) * 4;
+    auto kern = p.D <= 64    ? prefix_split_kernel<T, 2>
+                : p.D <= 128 ? prefix_split_kernel<T, 4>
+                             : prefix_split_kernel<T, 8>;
+    if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    kern<<<(unsigned)ctas, kPdThreads, smem, stream>>>(p, s, part);
     if (int rc = check_launch("prefix_split_kernel")) return rc;
   }
   prefix_join_kernel<T><<<(unsigned)(p.B * p.H), kPdThreads, 0, stream>>>(p, s, part);

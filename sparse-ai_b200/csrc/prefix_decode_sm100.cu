@@ -18,8 +18,7 @@
 // Persistent kernel, one CTA per SM, 12 warps (register split as in attn_fwd_sm100.cu):
 //   warp 11     scheduler: walks the CTA's range, reads page ids and row masks 32 pages per load,
 //               drops pages that no row attends and pushes tile descriptors into a ring;
-//   warp 8      TMA producer: K and V tiles in turn into one ring of kSlots tiles, Q tiles into two
-//               buffers;
+//   warps 8, 10 TMA producers: K (and Q, two buffers) and V tiles in turn into one ring of kSlots tiles;
 //   warp 9      MMA issuer.  Jobs (key tile x row tile) alternate between two lanes g = 0, 1, each
 //               with S[g] (fp32, 128 columns) and O[g] in TMEM: for job i it issues
 //               O[g] += P(i-2) V, then S[g] = Q K^T of job i, which may overwrite P(i-2) because
@@ -38,13 +37,15 @@ namespace {
 
 constexpr int kT = 128;          // rows of a row tile, keys of a key tile
 constexpr int kThreads = 384;
-constexpr int kProducerWarp = 8, kMmaWarp = 9, kTmemWarp = 10, kSchedWarp = 11;
-constexpr int kLaunchRegs = 168, kCtrlRegs = 72, kSoftmaxRegs = 216;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kVWarp = 10, kSchedWarp = 11;
+constexpr int kLaunchRegs = 168, kCtrlRegs = 120, kSoftmaxRegs = 192;
 static_assert(4 * 32 * kCtrlRegs + 8 * 32 * kSoftmaxRegs <= kThreads * kLaunchRegs,
               "register split exceeds the launch allocation");
 constexpr int kGroupThreads = 128;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kColS = 0, kColO = 256;  // S[g] at kColS + 128 g, O[g] at kColO + 128 g
+constexpr int kThin = 16;                   // rows up to which an item's products are transposed
+constexpr uint32_t kThinP = 8192;           // offset of a lane's P^T in the Q buffer of the same index
 constexpr int kMaxPpt = 8;                  // pages per key tile
 constexpr uint32_t kMaxSmem = 232448;
 constexpr float kRescaleThreshold = 8.0f;   // log2 units
@@ -56,7 +57,7 @@ constexpr int kMaxHeadWords = 8;            // query heads <= 256 (mask kernel)
 // tiles count by the share of their pages that some row attends.
 constexpr int kCostPair = 16, kCostOne = 11, kCostItem = 14;
 
-enum { F_FIRST = 1, F_LAST = 2, F_EMPTY = 4, F_END = 8, F_PAIR = 16, F_OWN = 32 };
+enum { F_FIRST = 1, F_LAST = 2, F_EMPTY = 4, F_END = 8, F_PAIR = 16, F_OWN = 32, F_THIN = 64 };
 
 struct TileDesc {
   int flags;
@@ -85,8 +86,8 @@ struct Layout {
   static constexpr int bFull = 0, bEmpty = bFull + kSlots, bQFull = bEmpty + kSlots, bQEmpty = bQFull + 2,
                        bSFull = bQEmpty + 2, bPFull = bSFull + 2, bODone = bPFull + 2, bOFree = bODone + 2,
                        bDFull = bOFree + 2, bDEmpty = bDFull + kDescs, bNum = bDEmpty + kDescs;
-  static constexpr uint32_t kMisc = kBars + bNum * 8;  // tmem slot, scan scratch
-  static constexpr uint32_t kBytes = kMisc + 192;
+  static constexpr uint32_t kMisc = kBars + bNum * 8;  // tmem slot, scan scratch, maxima of thin items
+  static constexpr uint32_t kBytes = kMisc + 192 + 2 * 4 * kThin * 4;
   static constexpr uint32_t kAlloc = kBytes + 1024 <= kMaxSmem ? kBytes + 1024 : kMaxSmem;
   static_assert(kBytes <= kMaxSmem, "prefix decode: shared-memory layout too large");
 };
@@ -142,7 +143,7 @@ struct Args {
 
 inline Split make_split(int64_t B, int64_t G, int64_t Hkv, int64_t page, int64_t Lp, int64_t L, int64_t D) {
   Split s;
-  s.nb = (int)(kT / G);
+  s.nb = (int)std::min<int64_t>(B, kT / G);
   s.row_tiles = (int)((B + s.nb - 1) / s.nb);
   s.units[0] = (int)(Hkv * (s.row_tiles / 2));
   s.units[1] = (int)(Hkv * (s.row_tiles & 1));
@@ -380,6 +381,69 @@ __global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const Pref
 // ---------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------
+// Warp maximum of a float, and a barrier of `threads` threads that returns the OR of a predicate.
+__device__ __forceinline__ float redux_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t threads, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)pred), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
+
+// 32 lanes x N consecutive 32-bit columns (N = 4, 8 or 16).
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ldn(uint32_t taddr, float (&v)[N]) {
+  if constexpr (N == 16) {
+    tmem_ld16(taddr, v);
+  } else if constexpr (N == 8) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+  } else {
+    uint32_t r[4];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_stn(uint32_t taddr, const uint32_t (&v)[N]) {
+  if constexpr (N == 16)
+    tmem_st16(taddr, v);
+  else if constexpr (N == 8)
+    tmem_st8(taddr, v);
+  else
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3])
+                 : "memory");
+}
+
 // Bounded waits as in common.cuh, counted in tries instead of timed: half the instructions at each
 // of the kernel's dozen waits, which matters where every role's code competes for the
 // instruction cache.  A try on a phase that stays incomplete suspends the thread for about 8 k
@@ -438,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     }
     for (int i = 0; i < L::kDescs; ++i) {
       mbar_init(&bars[L::bDFull + i], 1);
-      mbar_init(&bars[L::bDEmpty + i], 2 + 8);  // producer, MMA warp, 8 softmax warps
+      mbar_init(&bars[L::bDEmpty + i], 3 + 8);  // two producers, MMA warp, 8 softmax warps
     }
     fence_mbar_init();
     prefetch_tmap(&a.tm_k);
@@ -446,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     prefetch_tmap(&a.tm_q);
     prefetch_tmap(&a.tm_q1);
   }
-  if (warp == kTmemWarp) {
+  if (warp == kVWarp) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
@@ -571,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           tb = min(line.tiles_p, ta + hi - k);
           kvh = u / groups;
           const int rt = seg == 0 ? (u - kvh * groups) * 2 : S.row_tiles - 1;
-          flags = seg == 0 ? F_PAIR : 0;
+          flags = seg == 0 ? F_PAIR : S.B * S.G <= kThin ? F_THIN : 0;
           b0 = rt * S.nb;
           slot = (seg ? S.units[0] : 0) + u + (int)blockIdx.x;
           tokens = ptok;
@@ -587,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           kvh = r / t;
           ta = r - kvh * t;
           tb = min(t, ta + hi - k);
-          flags = F_OWN;
+          flags = F_OWN | (S.G <= kThin ? F_THIN : 0);
           b0 = b;
           slot = b * S.Hkv + kvh + (int)blockIdx.x;
           tokens = own_tok;
@@ -672,57 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         }
         if (flags & F_END) break;
       }
-    } else if (warp == kProducerWarp) {
-      // ---------------------------------------------------------------- TMA producer
-      const int dc = (S.D + 63) / 64;  // 64-column chunks
-      const int bn = S.bn;
-      uint32_t d = 0, seq = 0, nq = 0;
-      bool ok = true;
-      while (ok) {
-        const uint32_t ds = d % L::kDescs;
-        if (!wait_bar_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
-        const TileDesc& td = descs[ds];
-        const int flags = td.flags;
-        if (flags & F_END) break;
-        if (!(flags & F_EMPTY)) {
-          const int kvh = td.kvh, b0 = td.b0, n = td.n, t0 = td.t0;
-          if (flags & F_FIRST) {
-            const int tiles = flags & F_PAIR ? 2 : 1;
-            for (int i = 0; i < tiles && ok; ++i, ++nq) {
-              const uint32_t qb = nq & 1;
-              if (!(ok = wait_bar_warp(&bars[L::bQEmpty + qb], ((nq >> 1) & 1) ^ 1, st))) break;
-              if (elect_one()) {
-                unsigned char* dst = sm + L::kQ + qb * L::kTile;
-                const uint32_t rows = (uint32_t)((flags & F_OWN) ? S.G : S.nb * S.G);
-                mbar_arrive_expect_tx(&bars[L::bQFull + qb], rows * 128 * dc);
-                for (int c = 0; c < dc; ++c)
-                  tma_load_4d(dst + c * (kT * 128), (flags & F_OWN) ? &a.tm_q1 : &a.tm_q, &bars[L::bQFull + qb], c * 64,
-                              0, kvh, b0 + i * S.nb);
-              }
-              __syncwarp();
-            }
-          }
-          for (int kv = 0; kv < 2 && ok; ++kv, ++seq) {
-            const uint32_t sl = seq % L::kSlots;
-            if (!(ok = wait_bar_warp(&bars[L::bEmpty + sl], ((seq / L::kSlots) & 1) ^ 1, st))) break;
-            if (elect_one()) {
-              unsigned char* dst = sm + L::kRing + sl * L::kTile;
-              mbar_arrive_expect_tx(&bars[L::bFull + sl], (uint32_t)(n * bn * 128 * dc));
-#pragma unroll 1
-              for (int j = 0; j < n; ++j, dst += bn * 128) {
-                const int phys = td.phys[j];
-                for (int c = 0; c < dc; ++c)
-                  tma_load_4d(dst + c * (kT * 128), kv ? &a.tm_v : &a.tm_k, &bars[L::bFull + sl], c * 64, t0, kvh, phys);
-              }
-            }
-            __syncwarp();
-          }
-        }
-        if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
-        ++d;
-      }
-    } else if (warp == kTmemWarp) {
-      // ---------------------------------------------------------------- plan of the join
+      // ---- plan of the join, while the last tiles are under way
       // Where the partial states of the CTA's share of the requests are (lane = KV head): the CTAs
       // whose ranges hold the first and last tile of the prefix unit and of the own unit.
       const int per = (S.B + (int)gridDim.x - 1) / (int)gridDim.x;
@@ -759,17 +773,75 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         }
         cum += t;
       }
+    } else if (warp == kProducerWarp || warp == kVWarp) {
+      // ---------------------------------------------------------------- TMA producers
+      // Warp kProducerWarp loads Q and K, warp kVWarp V: issuing a tile's loads takes a warp up to 800
+      // cycles, and items of one tile (short own contexts) come every 2 k.
+      const bool is_v = warp == kVWarp;
+      const CUtensorMap* tm = is_v ? &a.tm_v : &a.tm_k;
+      const int dc = (S.D + 63) / 64;  // 64-column chunks
+      const int bn = S.bn;
+      uint32_t d = 0, seq = is_v ? 1 : 0, nq = 0;
+      bool ok = true;
+      while (ok) {
+        const uint32_t ds = d % L::kDescs;
+        if (!wait_bar_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
+        const TileDesc& td = descs[ds];
+        const int flags = td.flags;
+        if (flags & F_END) break;
+        if (!(flags & F_EMPTY)) {
+          const int kvh = td.kvh, b0 = td.b0, n = td.n, t0 = td.t0;
+          if (!is_v && (flags & F_FIRST)) {
+            const int tiles = flags & F_PAIR ? 2 : 1;
+            for (int i = 0; i < tiles && ok; ++i, ++nq) {
+              const uint32_t qb = nq & 1;
+              if (!(ok = wait_bar_warp(&bars[L::bQEmpty + qb], ((nq >> 1) & 1) ^ 1, st))) break;
+              if (elect_one()) {
+                unsigned char* dst = sm + L::kQ + qb * L::kTile;
+                const uint32_t rows = (uint32_t)((flags & F_OWN) ? S.G : S.nb * S.G);
+                mbar_arrive_expect_tx(&bars[L::bQFull + qb], rows * 128 * dc);
+                for (int c = 0; c < dc; ++c)
+                  tma_load_4d(dst + c * (kT * 128), (flags & F_OWN) ? &a.tm_q1 : &a.tm_q, &bars[L::bQFull + qb], c * 64,
+                              0, kvh, b0 + i * S.nb);
+              }
+              __syncwarp();
+            }
+          }
+          const uint32_t sl = seq % L::kSlots;
+          if (!ok || !wait_bar_warp(&bars[L::bEmpty + sl], ((seq / L::kSlots) & 1) ^ 1, st)) break;
+          if (elect_one()) {
+            unsigned char* dst = sm + L::kRing + sl * L::kTile;
+            mbar_arrive_expect_tx(&bars[L::bFull + sl], (uint32_t)(n * bn * 128 * dc));
+#pragma unroll 1
+            for (int j = 0; j < n; ++j, dst += bn * 128) {
+              const int phys = td.phys[j];
+              tma_load_4d(dst, tm, &bars[L::bFull + sl], 0, t0, kvh, phys);
+              if (dc > 1) tma_load_4d(dst + kT * 128, tm, &bars[L::bFull + sl], 64, t0, kvh, phys);
+            }
+          }
+          __syncwarp();
+          seq += 2;
+        }
+        if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
+        ++d;
+      }
     } else if (warp == kMmaWarp) {
       // ---------------------------------------------------------------- MMA issuer (one thread)
       if (elect_one()) {
       const int dk = (S.D + 15) / 16;  // K steps of Q K^T, and N / 16 of P V
       const uint32_t id_pv = idesc_f16(kT, dk * 16, BF16, false, true);
+      // thin items: S^T = K Q^T and O^T = V^T P^T, the keys (the head_dim) along the 128 lanes and the
+      // rows along 16 columns.  V^T spans 128 lanes in two 64-column chunks; where the tile has only
+      // one, the second half (any in-bounds data) lands in lanes that nobody reads.
+      constexpr uint32_t id_qk_t = idesc_f16(kT, kThin, BF16, false, false);
+      constexpr uint32_t id_pv_t = idesc_f16(kT, kThin, BF16, true, false);
+      constexpr uint32_t kVtLbo = DT == 128 ? kT * 128 : 1024;
       struct Job {
         uint32_t tile;  // key tile index: K in ring entry 2 tile, V in 2 tile + 1
         int vr;
         uint32_t bits;  // lane | J_*
       };
-      enum : uint32_t { J_FIRST = 2, J_LAST = 4, J_REL = 8 };
+      enum : uint32_t { J_FIRST = 2, J_LAST = 4, J_REL = 8, J_THIN = 16 };
       Job j0{}, j1{};  // pending P V products, j0 the older
       int np = 0;
       uint32_t d = 0, tile = 0, job = 0, nq = 0, pc[2] = {0, 0}, of[2] = {0, 0};
@@ -826,9 +898,19 @@ int in_item = 0;          // key tiles of the item so far
           uint64_t vd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), kT * 128, 1024);
           const uint32_t d_o = tmem + kColO + g * kT;
           uint32_t a_p = tmem + kColS + g * kT, acc = (j0.bits & J_FIRST) ? 0u : 1u;
+          if (j0.bits & J_THIN) {
+            vd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), kVtLbo, 1024);
+            uint64_t pd = smem_desc(smem_u32(sm + L::kQ + g * L::kTile + kThinP), 16, 1024);
 #pragma unroll 1
-          for (int kk = 0; kk < n16; kk += 16, a_p += 8, acc = 1u, vd = desc_add(vd, 16 * 128))
-            tc_mma_f16_ts(d_o, a_p, vd, id_pv, acc);
+            for (int kk = 0; kk < n16; kk += 16, acc = 1u, vd = desc_add(vd, 16 * 128)) {
+              tc_mma_f16(d_o, vd, pd, id_pv_t, acc);
+              pd = desc_add(pd, (kk & 48) == 48 ? kThin * 128 - 96 : 32);
+            }
+          } else {
+#pragma unroll 1
+            for (int kk = 0; kk < n16; kk += 16, a_p += 8, acc = 1u, vd = desc_add(vd, 16 * 128))
+              tc_mma_f16_ts(d_o, a_p, vd, id_pv, acc);
+          }
           if (j0.bits & J_REL) tc_commit(&bars[L::bEmpty + sl]);
           if (j0.bits & J_LAST) tc_commit(&bars[L::bODone + g]);
           j0 = j1;
@@ -842,13 +924,14 @@ int in_item = 0;          // key tiles of the item so far
           // ---- S[g] = Q K^T
           const uint32_t g = job & 1, sl = (2 * tile) % L::kSlots, qb = (nq + rts - left) & 1;
           tc_fence_after();
-          const uint32_t id_qk = idesc_f16(kT, (vr + 15) & ~15, BF16, false, false);
+          const bool thin = flags & F_THIN;
+          const uint32_t id_qk = thin ? id_qk_t : idesc_f16(kT, (vr + 15) & ~15, BF16, false, false);
           uint64_t qd = smem_desc(smem_u32(sm + L::kQ + qb * L::kTile), 16, 1024);
           uint64_t kd = smem_desc(smem_u32(sm + L::kRing + sl * L::kTile), 16, 1024);
           const uint32_t d_s = tmem + kColS + g * kT;
 #pragma unroll 1
           for (int kk = 0; kk < dk; ++kk) {
-            tc_mma_f16(d_s, qd, kd, id_qk, kk > 0 ? 1u : 0u);
+            tc_mma_f16(d_s, thin ? kd : qd, thin ? qd : kd, id_qk, kk > 0 ? 1u : 0u);
             const uint32_t step = (kk & 3) == 3 ? kT * 128 - 96 : 32;  // the next 16 columns
             qd = desc_add(qd, step);
             kd = desc_add(kd, step);
@@ -862,7 +945,7 @@ int in_item = 0;          // key tiles of the item so far
           j.tile = tile;
           j.vr = vr;
           j.bits = g | ((in_item == 0 || (rts == 1 && in_item == 1)) ? J_FIRST : 0u) | ((flags & F_LAST) ? J_LAST : 0u) |
-                   (left == 1 ? J_REL : 0u);
+                   (left == 1 ? J_REL : 0u) | (thin ? J_THIN : 0u);
           if (rts == 1 && (flags & F_LAST) && in_item > 0) {
             // the other lane's last product of the item is the one before this: pending, or issued
             if (np > 0) j0.bits |= J_LAST;
@@ -902,12 +985,161 @@ int in_item = 0;          // key tiles of the item so far
     bool had = false;
     int sub = 0;        // which of the slot's two states this group writes
     bool row_ok = false;
+    const int my_page = rl / S.bn;  // page of this key within a tile
+    float* s_max = reinterpret_cast<float*>(sm + L::kMisc + 192) + grp * 4 * kThin;  // [4 warps][kThin]
+    // V rows past the valid keys meet P = 0 in the product's last K step: they must be finite, so they
+    // are cleared (in a pair tile by both groups, with the same zeros).
+    auto clear_tail = [&](int vr) -> bool {
+      const uint32_t seq = 2 * (tile - 1) + 1, sl = seq % L::kSlots;
+      if (!wait_bar_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) return false;
+      unsigned char* vt = sm + L::kRing + sl * L::kTile;
+      const int units = (16 - (vr & 15)) * (DT / 8);
+#pragma unroll 1
+      for (int i = rl; i < units; i += kGroupThreads) {
+        const int rr = vr + i / (DT / 8), c = i % (DT / 8);
+        *reinterpret_cast<uint4*>(vt + (c >> 3) * (kT * 128) + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      return true;
+    };
+
+    // One thin item of nrow <= NR rows, from its first descriptor to its partial state.  Thread = key:
+    // its NR scores are one row of S^T, its probabilities NR columns of P^T; all threads of the group
+    // carry the rows' reference, each its own part of the rows' sums.
+    auto thin_item = [&](auto nr_, int nrow) -> bool {
+      constexpr int NR = decltype(nr_)::value;
+      float ref[NR], sum[NR];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        ref[r] = -INFINITY;
+        sum[r] = 0.f;
+      }
+      bool had_t = false;
+      int flags, slot;
+      do {
+        const uint32_t ds = d % L::kDescs;
+        if (!wait_bar_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) return false;
+        const TileDesc& td = descs[ds];
+        const int vr = td.vr;
+        flags = td.flags;
+        slot = td.slot;
+        const uint32_t on = a.masked ? td.mask[my_page & (kMaxPpt - 1)][0] : ~0u;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[L::bDEmpty + ds]);
+        ++d;
+        if (flags & F_EMPTY) break;
+        ++tile;
+        if ((int)(job++ & 1) != grp) continue;
+        const uint32_t gm = rl < vr ? on & ((1u << nrow) - 1u) : 0u;  // rows that attend this key
+        if (!wait_bar_warp(&bars[L::bSFull + grp], sc & 1, st)) return false;
+        ++sc;
+        tc_fence_after();
+        float x[NR];
+        tmem_ldn<NR>(lane_addr + col_s, x);
+        tmem_wait_ld();
+        // Scores in log2 units, -inf by selection where a row does not attend this key; each row's
+        // maximum over the warp's keys against the shared reference.
+        bool up = false;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          x[r] = (gm >> r) & 1u ? x[r] * sc2 : -INFINITY;
+          const float wm = redux_max(x[r]);
+          up |= wm > ref[r] + kRescaleThreshold || (ref[r] == -INFINITY && wm != -INFINITY);
+          if (lane == 0) s_max[quarter * kThin + r] = wm;
+        }
+        if (named_bar_or(1 + grp, kGroupThreads, up)) {
+          // some row's reference moves, to its maximum over the tile's keys; the sums and O^T (a row is a
+          // column of it; S(i) being complete implies that the lane's last product is) follow
+          float f[NR];
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            f[r] = 1.f;
+            const float mt = fmaxf(fmaxf(s_max[r], s_max[kThin + r]), fmaxf(s_max[2 * kThin + r], s_max[3 * kThin + r]));
+            if (mt > ref[r] + kRescaleThreshold || (ref[r] == -INFINITY && mt != -INFINITY)) {
+              f[r] = ref[r] == -INFINITY ? 0.f : fast_exp2(ref[r] - mt);
+              sum[r] *= f[r];
+              ref[r] = mt;
+            }
+          }
+          named_bar_sync(1 + grp, kGroupThreads);  // s_max is read
+          if (had_t) {
+            float o[NR];
+            uint32_t u[NR];
+            tmem_ldn<NR>(lane_addr + col_o, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int r = 0; r < NR; ++r) u[r] = f[r] == 0.f ? 0u : __float_as_uint(o[r] * f[r]);
+            tmem_stn<NR>(lane_addr + col_o, u);
+            tmem_wait_st();
+          }
+        }
+        // P^T: a row's 128 keys as two 128-byte swizzled rows of 64, in the unused part of a Q buffer
+        unsigned char* pt = sm + L::kQ + grp * L::kTile + kThinP + (rl >> 6) * (kThin * 128) + (rl & 7) * 2;
+        const int unit = (rl & 63) >> 3;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float e = ref[r] == -INFINITY ? 0.f : fast_exp2(x[r] - ref[r]);
+          sum[r] += e;
+          *reinterpret_cast<uint16_t*>(pt + r * 128 + ((unit ^ (r & 7)) << 4)) = (uint16_t)pack2(e, 0.f, BF16);
+        }
+        fence_proxy_async_smem();
+        if (__builtin_expect(vr & 15, 0) && !clear_tail(vr)) return false;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[L::bPFull + grp]);
+        had_t = true;
+      } while (!(flags & F_LAST));
+      // ---- the item's partial state: each row's sum over the keys; O^T's lane d is column d of every row
+      const bool own = flags & F_OWN;
+      const int rows = own ? G : kT;
+      const int64_t state = (int64_t)slot * 2 + grp;
+      float2* ml = (own ? a.w.ml_o : a.w.ml_p) + state * rows;
+      float* acc = reinterpret_cast<float*>((own ? a.w.acc_o : a.w.acc_p) + state * D4 * rows);
+      if (!had_t) {
+        if (rl < nrow) ml[rl] = make_float2(-INFINITY, 0.f);
+        return true;
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float l = sum[r];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) s_max[quarter * kThin + r] = l;
+      }
+      if (!wait_bar_warp(&bars[L::bODone + grp], od & 1, st)) return false;
+      ++od;
+      tc_fence_after();
+      float o[NR];
+      tmem_ldn<NR>(lane_addr + col_o, o);
+      tmem_wait_ld();
+      tc_fence_before();
+      named_bar_sync(1 + grp, kGroupThreads);  // s_max is complete, O^T is read
+      if (lane == 0) mbar_arrive(&bars[L::bOFree + grp]);
+      float m = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        if (r < nrow && rl < S.D) acc[((int64_t)(rl >> 2) * rows + r) * 4 + (rl & 3)] = o[r];
+        if (r == rl) m = ref[r];
+      }
+      if (rl < nrow) ml[rl] = make_float2(m, s_max[rl] + s_max[kThin + rl] + s_max[2 * kThin + rl] + s_max[3 * kThin + rl]);
+      named_bar_sync(1 + grp, kGroupThreads);  // s_max is read: the next tile may write it
+      return true;
+    };
+
     while (true) {
       const uint32_t ds = d % L::kDescs;
       if (!wait_bar_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
       const TileDesc& td = descs[ds];
       const int flags = td.flags, vr = td.vr, slot = td.slot, n = td.n;
       if (flags & F_END) break;
+      if (flags & F_THIN) {  // a whole item; its first descriptor is not released yet
+        const int nrow = flags & F_OWN ? G : S.B * G;
+        const bool ok = nrow <= 4   ? thin_item(std::integral_constant<int, 4>{}, nrow)
+                        : nrow <= 8 ? thin_item(std::integral_constant<int, 8>{}, nrow)
+                                    : thin_item(std::integral_constant<int, 16>{}, nrow);
+        if (!ok) break;
+        continue;
+      }
       const bool pair = flags & F_PAIR, own = flags & F_OWN, empty = flags & F_EMPTY;
       if (flags & F_FIRST) {
         sub = pair ? ((int)(job & 1) ^ grp) : grp;
@@ -1077,18 +1309,7 @@ int in_item = 0;          // key tiles of the item so far
           tmem_wait_st();
         }
         if (__builtin_expect(vr & 15, 0)) {
-          // V rows past the valid keys meet P = 0 in the product's last K step: they must be finite, so
-          // they are cleared (in a pair tile by both groups, with the same zeros)
-          const uint32_t seq = 2 * (tile - 1) + 1, sl = seq % L::kSlots;
-          if (!wait_bar_warp(&bars[L::bFull + sl], (seq / L::kSlots) & 1, st)) break;
-          unsigned char* vt = sm + L::kRing + sl * L::kTile;
-          const int units = (16 - (vr & 15)) * (DT / 8);
-#pragma unroll 1
-          for (int i = rl; i < units; i += kGroupThreads) {
-            const int rr = vr + i / (DT / 8), c = i % (DT / 8);
-            *reinterpret_cast<uint4*>(vt + (c >> 3) * (kT * 128) + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
+          if (!clear_tail(vr)) break;
         }
         tc_fence_before();
         __syncwarp();
@@ -1131,7 +1352,7 @@ int in_item = 0;          // key tiles of the item so far
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kTmemWarp) {
+  if (warp == kVWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
@@ -1368,7 +1589,7 @@ int launch_prefix_fast(const PrefixParams& p, int dtype, void* workspace, cudaSt
   // cells is one whose prefix is cut finely, with many states to join.
   const int64_t cells = p.G * p.D / 4, all = cells * p.B * p.Hkv, fill = (int64_t)device_sm_count() * 1024;
   int groups = 1;
-  while (groups < 16 && all * groups * 2 <= fill) groups *= 2;
+  while (groups < 16 && (all * groups * 2 <= fill || kCombThreads / groups >= 2 * cells)) groups *= 2;
   const int cpb = kCombThreads / groups;
   const dim3 grid((unsigned)(p.B * p.Hkv), (unsigned)((cells + cpb - 1) / cpb)), block(kCombThreads);
   if (bf)

@@ -271,108 +271,141 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
 // level; a ballot per page is the page's mask word.  Integer compares of a few MB that sit in L2.
 constexpr int kMaskWarps = 4;
 
+struct MaskArgs {
+  Split s;
+  Ws w;
+  const int32_t* ppages;
+  const int32_t* bt;
+  int64_t bts0, bts1;
+  const int32_t* ctx;
+  const int32_t* plen_dev;
+  const void* router;
+  int64_t rs[3];
+  const void* qrouter;
+  int64_t qrs[3];
+  int plen, num_pages, q64, r, local, sink, H;
+  int prefix_tasks, tasks;
+};
+
 template <typename RT>
-__global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const PrefixParams p, const Split s, const Ws w,
-                                                                     int64_t prefix_tasks, int64_t own_tasks) {
+__global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const __grid_constant__ MaskArgs a) {
   __shared__ uint32_t s_bits[kMaskWarps][kMaskPages][kMaxHeadWords];
   pdl_trigger();
+  const Split& s = a.s;
+  const Ws& w = a.w;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const RT* router = static_cast<const RT*>(p.router);
-  const int64_t pre_pages = (prefix_tokens(p) + p.page - 1) / p.page;
-  const int r = (int)p.r;
-  // bits u = 0..15: whether page u's vector equals the row's on the first r levels
-  auto match = [&](int phys, int64_t b, int64_t h) -> uint32_t {
-    uint32_t bits = (1u << kMaskPages) - 1u;
-    for (int lv = 0; lv < r; ++lv) {
-      const int64_t qv = load_any_i64(p.qrouter, p.qrouter_dtype, b * p.qrs[0] + h * p.qrs[1] + lv * p.qrs[2]);
-      RT rv[kMaskPages];
+  const RT* router = static_cast<const RT*>(a.router);
+  const int pre_pages = (pre_tokens(s, a.plen_dev, a.plen) + s.page - 1) / s.page;
+  // bits u = 0..15: whether page u's vector equals the row's on the first r levels; 4 pages x 4 levels
+  // in flight (all 16 pages unrolled made 47 KB of code that waited for its instructions)
+  auto match = [&](int phys, int b, int h) -> uint32_t {
+    uint32_t bits = 0;
+    const RT* rh = router + h * a.rs[1];
+    const int64_t qo = b * a.qrs[0] + h * a.qrs[1];
+#pragma unroll 1
+    for (int u0 = 0; u0 < kMaskPages; u0 += 4) {
+      uint32_t on = 15u;
+#pragma unroll 1
+      for (int lv0 = 0; lv0 < a.r; lv0 += 4) {
+        RT v[4][4];
+        int64_t q[4];
 #pragma unroll
-      for (int u = 0; u < kMaskPages; ++u)
-        rv[u] = __ldg(router + (int64_t)__shfl_sync(0xffffffffu, phys, u) * p.rs[0] + h * p.rs[1] + lv * p.rs[2]);
+        for (int k = 0; k < 4; ++k) {  // levels past r repeat the last
+          const int lv = min(lv0 + k, a.r - 1);
+          q[k] = load_any_i64(a.qrouter, a.q64 ? SA_I64 : SA_I32, qo + lv * a.qrs[2]);
 #pragma unroll
-      for (int u = 0; u < kMaskPages; ++u)
-        if ((int64_t)rv[u] != qv) bits &= ~(1u << u);
+          for (int u = 0; u < 4; ++u)
+            v[u][k] = __ldg(rh + (int64_t)__shfl_sync(0xffffffffu, phys, u0 + u) * a.rs[0] + lv * a.rs[2]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if ((int64_t)v[u][k] != q[k]) on &= ~(1u << u);
+      }
+      bits |= on << u0;
     }
     return bits;
   };
-  for (int64_t task = (int64_t)blockIdx.x * kMaskWarps + warp; task < prefix_tasks + own_tasks;
-       task += (int64_t)gridDim.x * kMaskWarps) {
-    if (task < prefix_tasks) {
-      int64_t x = task;
-      const int64_t chunks = (p.Lp + kMaskPages - 1) / kMaskPages;
-      const int64_t l0 = (x % chunks) * kMaskPages;
-      x /= chunks;
-      const int word = (int)(x % 4);
-      x /= 4;
-      const int64_t rt = x % s.row_tiles, g = x / s.row_tiles;
+  for (int task = (int)blockIdx.x * kMaskWarps + warp; task < a.tasks; task += (int)gridDim.x * kMaskWarps) {
+    if (task < a.prefix_tasks) {
+      const int chunks = prefix_chunks(s);
+      int x = task / chunks;
+      const int chunk = task - x * chunks, l0 = chunk * kMaskPages, word = x & 3;
+      x >>= 2;
+      const int g = x / s.row_tiles, rt = x - g * s.row_tiles;
       const bool counted = word == 0 && rt == s.row_tiles - 1 && (s.row_tiles & 1);
-      if (l0 >= pre_pages) {
-        if (counted && lane == 0) w.cnt_p[g * chunks + l0 / kMaskPages] = 0;
-        continue;
+      uint32_t bits = 0;
+      const int row = word * 32 + lane, rb = row / s.G, b = rt * s.nb + rb;
+      const bool live = row < s.nb * s.G && b < s.B;
+      int n = pre_pages;
+      if (l0 < pre_pages && word * 32 < s.nb * s.G) {
+        int phys = lane < kMaskPages && l0 + lane < pre_pages ? a.ppages[l0 + lane] : 0;
+        if (phys < 0 || phys >= a.num_pages) phys = 0;  // dropped by the scheduler
+        if (a.local > 0 && live) n += (tokens_in(a.ctx[b], s.L, s.page) + s.page - 1) / s.page;
+        bits = match(phys, live ? b : 0, live ? g * s.G + row - rb * s.G : 0);
       }
-      const int row = word * 32 + lane;
-      const int64_t b = rt * s.nb + row / p.G, h = g * p.G + row % p.G;
-      const bool live = row < s.nb * p.G && b < p.B;
-      int phys = lane < kMaskPages && l0 + lane < pre_pages ? p.ppages[l0 + lane] : 0;
-      if (phys < 0 || phys >= p.num_pages) phys = 0;  // dropped by the scheduler
-      uint32_t bits = match(phys, live ? b : 0, live ? h : 0);
-      const int64_t n = pre_pages + (live ? (own_tokens(p, b) + p.page - 1) / p.page : 0);
+      // forced pages: the sink, and the last `local` of the row's n pages
+      uint32_t forced = a.sink && l0 == 0 ? 1u : 0u;
+      const int first = n - a.local - l0;  // first forced page of this chunk
+      if (a.local > 0 && first < kMaskPages) forced |= ~0u << max(0, first);
+      bits = live ? bits | forced : 0u;
       int count = 0;
+#pragma unroll 1
       for (int u = 0; u < kMaskPages; ++u) {
-        const int64_t l = l0 + u;
-        const bool on = ((bits >> u) & 1u) || (p.sink && l == 0) || l >= n - p.local_blocks;
-        const uint32_t m = __ballot_sync(0xffffffffu, live && on);
-        if (l < pre_pages) {
+        const uint32_t m = __ballot_sync(0xffffffffu, (bits >> u) & 1u);
+        if (l0 + u < pre_pages) {
           count += m != 0u;
-          if (lane == 0) w.mask_p[((g * s.row_tiles + rt) * p.Lp + l) * 4 + word] = m;
+          if (lane == 0) w.mask_p[(((int64_t)g * s.row_tiles + rt) * s.Lp + l0 + u) * 4 + word] = m;
         }
       }
-      if (counted && lane == 0) w.cnt_p[g * chunks + l0 / kMaskPages] = count;
+      if (counted && lane == 0) w.cnt_p[g * chunks + chunk] = count;
     } else {
-      int64_t x = task - prefix_tasks;
-      const int64_t chunks = (p.L + kMaskPages - 1) / kMaskPages;
-      const int64_t l0 = (x % chunks) * kMaskPages, b = x / chunks;
-      const int64_t pages = (own_tokens(p, b) + p.page - 1) / p.page;
+      const int t = task - a.prefix_tasks, chunks = own_chunks(s), b = t / chunks, l0 = (t - b * chunks) * kMaskPages;
+      const int pages = (tokens_in(a.ctx[b], s.L, s.page) + s.page - 1) / s.page;
       if (l0 >= pages) {
-        if (lane == 0) w.cnt_o[task - prefix_tasks] = 0;
+        if (lane == 0) w.cnt_o[t] = 0;
         continue;
       }
-      int count = 0;  // (page, KV head) pairs that some head attends
-      int phys = lane < kMaskPages && l0 + lane < pages ? p.bt[b * p.bts[0] + (l0 + lane) * p.bts[1]] : 0;
-      if (phys < 0 || phys >= p.num_pages) phys = 0;
-      const int HW = (int)((p.H + 31) / 32);
+      int phys = lane < kMaskPages && l0 + lane < pages ? a.bt[b * a.bts0 + (l0 + lane) * a.bts1] : 0;
+      if (phys < 0 || phys >= a.num_pages) phys = 0;
+      uint32_t forced = a.sink && pre_pages + l0 == 0 ? 1u : 0u;
+      const int first = pages - a.local - l0;
+      if (a.local > 0 && first < kMaskPages) forced |= ~0u << max(0, first);
+      const int HW = (a.H + 31) / 32;
       for (int hw = 0; hw < HW; ++hw) {
-        const int64_t h = hw * 32 + lane;
-        const bool live = h < p.H;
-        const uint32_t bits = match(phys, b, live ? h : 0);
+        const int h = hw * 32 + lane;
+        const bool live = h < a.H;
+        uint32_t bits = match(phys, b, live ? h : 0) | forced;
+        if (!live) bits = 0;
+#pragma unroll 1
         for (int u = 0; u < kMaskPages; ++u) {
-          const int64_t l = l0 + u;
-          const bool on = ((bits >> u) & 1u) || (p.sink && pre_pages + l == 0) || l >= pages - p.local_blocks;
-          const uint32_t m = __ballot_sync(0xffffffffu, live && on);
+          const uint32_t m = __ballot_sync(0xffffffffu, (bits >> u) & 1u);
           if (lane == 0) s_bits[warp][u][hw] = m;
         }
       }
       __syncwarp();
       // each KV head's G bits out of the H
-      const int per = (int)p.Hkv * w.WO;
+      int count = 0;  // (page, KV head) pairs that some head attends
+      const int per = s.Hkv * w.WO;
       for (int i = lane; i < kMaskPages * per; i += 32) {
-        const int u = i / per, g = (i % per) / w.WO, wd = i % w.WO;
+        const int u = i / per, gw = i - u * per, g = gw / w.WO, wd = gw - g * w.WO;
         if (l0 + u >= pages) continue;
-        const int first = g * (int)p.G + wd * 32, cnt = min(32, (int)p.G - wd * 32);
+        const int first_h = g * s.G + wd * 32, cnt = min(32, s.G - wd * 32);
         uint32_t m = 0;
         if (cnt > 0) {
-          const int q = first >> 5, off = first & 31;
+          const int q = first_h >> 5;
           uint64_t v = s_bits[warp][u][q];
           if (q + 1 < HW) v |= (uint64_t)s_bits[warp][u][q + 1] << 32;
-          m = (uint32_t)(v >> off);
+          m = (uint32_t)(v >> (first_h & 31));
           if (cnt < 32) m &= (1u << cnt) - 1u;
         }
-        w.mask_o[((b * p.Hkv + g) * p.L + l0 + u) * w.WO + wd] = m;
+        w.mask_o[(((int64_t)b * s.Hkv + g) * s.L + l0 + u) * w.WO + wd] = m;
         count += m != 0u;
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
-      if (lane == 0) w.cnt_o[task - prefix_tasks] = count;
+      if (lane == 0) w.cnt_o[t] = count;
       __syncwarp();
     }
   }
@@ -1361,7 +1394,7 @@ int in_item = 0;          // key tiles of the item so far
 // ---------------------------------------------------------------------------------------
 // join of the partial states, one CTA per (request, KV head)
 // ---------------------------------------------------------------------------------------
-constexpr int kCombThreads = 256;
+constexpr int kCombThreads = 256;  // at most
 
 // Row (b, h) by itself, one warp: for rows whose joined state is not finite.  In the tensor-core
 // product a page's V meets every row of the tile, with weight 0 where the row does not attend
@@ -1420,7 +1453,7 @@ __global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const __gr
   __shared__ unsigned s_bad[4];  // rows (of the group) to compute again
   const int G = s.G, D4 = s.D / 4, tid = threadIdx.x;
   const int b = blockIdx.x / s.Hkv, g = blockIdx.x - b * s.Hkv;
-  const int CG = kCombThreads / cpb;  // thread groups over the states
+  const int CG = (int)blockDim.x / cpb;  // thread groups over the states
   const int cg = tid / cpb, ci = tid - cg * cpb;
   if (tid < 4) s_bad[tid] = 0;
   pdl_wait();
@@ -1486,7 +1519,7 @@ __global__ void __launch_bounds__(kCombThreads) prefix_combine_kernel(const __gr
   }
   __syncthreads();
   // (the CTA's cells of head r are the columns 4 c with cell0 <= c G + r < cell0 + cpb)
-  for (int r = tid >> 5; r < G; r += kCombThreads / 32)
+  for (int r = tid >> 5; r < G; r += (int)blockDim.x / 32)
     if ((s_bad[r >> 5] >> (r & 31)) & 1u)
       exact_row<T>(p, b, g * G + r, scale2, 4 * max(0, (cell0 - r + G - 1) / G),
                    4 * min(D4, max(0, (cell0 + cpb - r + G - 1) / G)));
@@ -1569,14 +1602,35 @@ int launch_prefix_fast(const PrefixParams& p, int dtype, void* workspace, cudaSt
   if (!rc) rc = make_tmap_4d(&a.tm_v, p.vc, dtype, p.num_pages, p.Hkv, p.page, p.D, p.vs, 64, (uint32_t)a.s.bn);
   if (rc) return fail(SA_ELAUNCH, std::string("prefix decode tensor maps: ") + sa_last_error());
   if (a.masked) {
-    const int64_t pt = p.Hkv * a.s.row_tiles * 4 * ((p.Lp + kMaskPages - 1) / kMaskPages);
-    const int64_t ot = p.B * ((p.L + kMaskPages - 1) / kMaskPages);
-    const int grid = (int)std::max<int64_t>(
-        1, std::min<int64_t>((pt + ot + kMaskWarps - 1) / kMaskWarps, (int64_t)device_sm_count() * 8));
+    MaskArgs ma{};
+    ma.s = a.s;
+    ma.w = a.w;
+    ma.ppages = p.ppages;
+    ma.bt = p.bt;
+    ma.bts0 = p.bts[0];
+    ma.bts1 = p.bts[1];
+    ma.ctx = p.ctx;
+    ma.plen_dev = p.plen_dev;
+    ma.plen = (int)p.plen;
+    ma.num_pages = (int)p.num_pages;
+    ma.router = p.router;
+    ma.qrouter = p.qrouter;
+    for (int i = 0; i < 3; ++i) {
+      ma.rs[i] = p.rs[i];
+      ma.qrs[i] = p.qrs[i];
+    }
+    ma.q64 = p.qrouter_dtype == SA_I64;
+    ma.r = (int)p.r;
+    ma.local = (int)std::min<int64_t>(p.local_blocks, INT32_MAX / 2);
+    ma.sink = p.sink;
+    ma.H = (int)p.H;
+    ma.prefix_tasks = (int)(p.Hkv * a.s.row_tiles * 4 * prefix_chunks(a.s));
+    ma.tasks = ma.prefix_tasks + (int)(p.B * own_chunks(a.s));
+    const int grid = std::max(1, std::min((ma.tasks + kMaskWarps - 1) / kMaskWarps, device_sm_count() * 8));
     if (p.router_dtype == SA_I64)
-      prefix_mask_kernel<int64_t><<<grid, kMaskWarps * 32, 0, stream>>>(p, a.s, a.w, pt, ot);
+      prefix_mask_kernel<int64_t><<<grid, kMaskWarps * 32, 0, stream>>>(ma);
     else
-      prefix_mask_kernel<int32_t><<<grid, kMaskWarps * 32, 0, stream>>>(p, a.s, a.w, pt, ot);
+      prefix_mask_kernel<int32_t><<<grid, kMaskWarps * 32, 0, stream>>>(ma);
     if ((rc = check_launch("prefix_mask_kernel"))) return rc;
   }
   const bool bf = dtype == SA_BF16;
@@ -1589,9 +1643,9 @@ int launch_prefix_fast(const PrefixParams& p, int dtype, void* workspace, cudaSt
   // cells is one whose prefix is cut finely, with many states to join.
   const int64_t cells = p.G * p.D / 4, all = cells * p.B * p.Hkv, fill = (int64_t)device_sm_count() * 1024;
   int groups = 1;
-  while (groups < 16 && (all * groups * 2 <= fill || kCombThreads / groups >= 2 * cells)) groups *= 2;
-  const int cpb = kCombThreads / groups;
-  const dim3 grid((unsigned)(p.B * p.Hkv), (unsigned)((cells + cpb - 1) / cpb)), block(kCombThreads);
+  while (groups < 16 && all * groups * 2 <= fill) groups *= 2;
+  const int cpb = (int)std::min<int64_t>(kCombThreads / groups, (cells + 31) / 32 * 32);
+  const dim3 grid((unsigned)(p.B * p.Hkv), (unsigned)((cells + cpb - 1) / cpb)), block((unsigned)(cpb * groups));
   if (bf)
     return launch_dependent(prefix_combine_kernel<__nv_bfloat16>, grid, block, 0, stream, "prefix_combine_kernel", p, a.s,
                             a.w, a.scale2, cpb);

@@ -1012,12 +1012,13 @@ int in_item = 0;          // key tiles of the item so far
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t col_s = kColS + grp * kT, col_o = kColO + grp * kT;
     const float sc2 = a.scale2;
-    const int G = S.G, D4 = S.D / 4;
+    const int G = S.G;
     uint32_t d = 0, job = 0, tile = 0, sc = 0, od = 0;
     float m_used = -INFINITY, l_sum = 0.f;
     bool had = false;
     int sub = 0;        // which of the slot's two states this group writes
     bool row_ok = false;
+    int slot = 0;
     const int my_page = rl / S.bn;  // page of this key within a tile
     float* s_max = reinterpret_cast<float*>(sm + L::kMisc + 192) + grp * 4 * kThin;  // [4 warps][kThin]
     // V rows past the valid keys meet P = 0 in the product's last K step: they must be finite, so they
@@ -1127,7 +1128,7 @@ int in_item = 0;          // key tiles of the item so far
       const int rows = own ? G : kT;
       const int64_t state = (int64_t)slot * 2 + grp;
       float2* ml = (own ? a.w.ml_o : a.w.ml_p) + state * rows;
-      float* acc = reinterpret_cast<float*>((own ? a.w.acc_o : a.w.acc_p) + state * D4 * rows);
+      float* acc = reinterpret_cast<float*>((own ? a.w.acc_o : a.w.acc_p) + state * (S.D / 4) * rows);
       if (!had_t) {
         if (rl < nrow) ml[rl] = make_float2(-INFINITY, 0.f);
         return true;
@@ -1163,7 +1164,8 @@ int in_item = 0;          // key tiles of the item so far
       const uint32_t ds = d % L::kDescs;
       if (!wait_bar_warp(&bars[L::bDFull + ds], (d / L::kDescs) & 1, st)) break;
       const TileDesc& td = descs[ds];
-      const int flags = td.flags, vr = td.vr, slot = td.slot, n = td.n;
+      const int flags = td.flags, vr = td.vr, n = td.n;
+      if (flags & F_FIRST) slot = td.slot;
       if (flags & F_END) break;
       if (flags & F_THIN) {  // a whole item; its first descriptor is not released yet
         const int nrow = flags & F_OWN ? G : S.B * G;
@@ -1357,7 +1359,7 @@ int in_item = 0;          // key tiles of the item so far
       const int rows = own ? G : kT;
       const int64_t state = (int64_t)slot * 2 + sub;
       float2* ml = (own ? a.w.ml_o : a.w.ml_p) + state * rows;
-      float4* acc = (own ? a.w.acc_o : a.w.acc_p) + state * D4 * rows;
+      float4* acc = (own ? a.w.acc_o : a.w.acc_p) + state * (S.D / 4) * rows;
       if (row_ok) ml[rl] = make_float2(had ? m_used : -INFINITY, l_sum);
       if (had) {
         if (!wait_bar_warp(&bars[L::bODone + grp], od & 1, st)) break;
@@ -1367,13 +1369,13 @@ int in_item = 0;          // key tiles of the item so far
           const bool put = row_ok && (m_used != -INFINITY || l_sum != 0.f);
           float4* dst = acc + rl;
 #pragma unroll 1
-          for (int c = 0; c * 8 < D4; ++c, dst += 8 * rows) {
+          for (int c = 0; c * 32 < S.D; ++c, dst += 8 * rows) {
             float o[32];
             tmem_ld32(lane_addr + col_o + c * 32, o);
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (put && c * 8 + i < D4) dst[i * rows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              if (put && c * 32 + 4 * i < S.D) dst[i * rows] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
         tc_fence_before();

@@ -51,11 +51,14 @@ constexpr uint32_t kMaxSmem = 232448;
 constexpr float kRescaleThreshold = 8.0f;   // log2 units
 constexpr int kMaxHeadWords = 8;            // query heads <= 256 (mask kernel)
 
-// Cost of one key tile in the split of the work over CTAs, in units of about 250 cycles (traced): a
-// pair tile, a tile of either other kind, and what an item costs besides its tiles (fill, drain and
-// partial states; of a pair item twice that), spread over its tiles.  With routing, own and single
-// tiles count by the share of their pages that some row attends.
-constexpr int kCostPair = 16, kCostOne = 11, kCostItem = 14;
+// Relative cost of one key tile in the split of the work over CTAs: a pair tile (about 4000 cycles),
+// a tile of either other kind, and what an item costs besides its tiles (fill, drain and partial
+// states; of a pair item twice that), spread over its tiles.  With routing, own and single tiles
+// count by the share of their pages that some row attends.  Fitted by timing: 256 requests on a
+// prefix of 32768 and up to 768 own tokens take 195 us with these, 230 with 16 / 11 / 14 (the traced
+// cycles of a tile on an idle GPU: beside pair tiles, own tiles have more of HBM to themselves)
+// and 228 with 24 / 9 / 9.
+constexpr int kCostPair = 18, kCostOne = 9, kCostItem = 6;
 
 enum { F_FIRST = 1, F_LAST = 2, F_EMPTY = 4, F_END = 8, F_PAIR = 16, F_OWN = 32, F_THIN = 64 };
 

@@ -31,6 +31,7 @@ from .paged_tables import (
     paged_kv_write,
     release_paged_requests,
 )
+from .shared_prefix import SharedPrefixCache
 
 __all__ = [
     "HAS_TRITON",
@@ -50,4 +51,5 @@ __all__ = [
     "build_paged_tables",
     "release_paged_requests",
     "paged_kv_write",
+    "SharedPrefixCache",
 ]

@@ -38,8 +38,8 @@ struct WriteParams {
 // flight while the slots arrive and are divided into page and row, once per token.
 //
 // Bound by HBM: 2 T Hkv D elements in and as many out.  32768 tokens of 8 heads of 128 bf16 (268 MB
-// of traffic): one token per CTA 95 us, 8 tokens 48 us (5.6 TB/s; a plain copy runs at 6.5).  Below about 8 tokens per SM the CTAs would not cover the GPU, and one token per CTA ends
-// sooner.
+// of traffic): one token per CTA 95 us, 8 tokens 48 us (5.6 TB/s; a plain copy runs at 6.5).  Below
+// about 8 tokens per SM the CTAs would not cover the GPU, and one token per CTA ends sooner.
 template <typename V, int kTok>
 __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteParams p) {
   __shared__ int64_t s_page[kTok], s_row[kTok];  // page -1: no slot

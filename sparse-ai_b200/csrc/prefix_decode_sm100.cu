@@ -7,25 +7,46 @@
 //   pair    prefix tiles against two row tiles at once (2 nb requests): each K/V tile that is
 //           loaded serves 256 rows;
 //   single  prefix tiles against one row tile (the last one where their number is odd);
-//   own     each request's own pages against its G rows, in the same MMA tile shape: 128 - G
-//           rows of the product are unused, but a 128 x 128 tile pair of products takes about 1100
-//           cycles against the 2700 in which one SM's share of HBM delivers the tile's 64 KB.
+//   own     each request's own pages against its G rows.
 // CTA i takes the weighted range [i W / n, (i + 1) W / n) of that line (computed on the device:
-// lengths live there), so every SM gets the same number of tiles whatever the lengths, and a unit
-// (KV head and rows) is cut only where a range ends.  Each (unit, CTA) piece leaves one partial
-// state per row (max, sum, accumulator), which prefix_combine_kernel joins.
+// lengths live there), so every SM gets the same work whatever the lengths, and a unit (KV head
+// and rows) is cut only where a range ends.  Each (unit, CTA) piece leaves one partial state per
+// row (max, sum, accumulator), which prefix_combine_kernel joins.
 //
-// Persistent kernel, one CTA per SM, 12 warps (register split as in attn_fwd_sm100.cu):
+// Items of at most kThin = 16 rows (own items of groups up to 16, the prefix of a few requests)
+// turn the products around: S^T = K Q^T and O^T = V^T P^T, keys (then columns of V) along the 128
+// lanes and the rows along 16 columns.  A tile then costs the tensor pipe an eighth, and its softmax
+// NR <= 16 exponentials per thread in place of 128 in G of 128 threads: own items of up to 768 tokens
+// of 256 requests went from 127 to 90 us.  More rows than that stay in the 128-row form, where rows
+// need no exchange between threads.
+//
+// Up to three kernels, chained by programmatic dependent launch: prefix_mask_kernel (with
+// routing only) says which rows attend each page, prefix_sm100_kernel leaves partial states,
+// prefix_combine_kernel joins them.  The second is persistent, one CTA per SM, 12 warps (register
+// split as in attn_fwd_sm100.cu):
 //   warp 11     scheduler: walks the CTA's range, reads page ids and row masks 32 pages per load,
-//               drops pages that no row attends and pushes tile descriptors into a ring;
-//   warps 8, 10 TMA producers: K (and Q, two buffers) and V tiles in turn into one ring of kSlots tiles;
-//   warp 9      MMA issuer.  Jobs (key tile x row tile) alternate between two lanes g = 0, 1, each
-//               with S[g] (fp32, 128 columns) and O[g] in TMEM: for job i it issues
+//               drops pages that no row attends and pushes tile descriptors into a ring; then its
+//               share of the join's plan (where each row's partial states are);
+//   warps 8, 10 TMA producers, of Q (two buffers) and K, and of V, into one ring of kSlots tiles;
+//   warp 9      MMA issuer, one thread.  Jobs (key tile x row tile) alternate between two lanes
+//               g = 0, 1, each with S[g] (fp32, 128 columns) and O[g] in TMEM: for job i it issues
 //               O[g] += P(i-2) V, then S[g] = Q K^T of job i, which may overwrite P(i-2) because
 //               the tensor pipe takes one thread's products in order;
-//   warps 0-7   two softmax warpgroups, one per lane; thread = row: masks by selection, running
-//               maximum (O rescaled in TMEM only when it grows by more than 2^8), exp2, P to TMEM
-//               over S's columns (A operand of the next product), partials to global memory.
+//   warps 0-7   two softmax warpgroups, one per lane; thread = row (thin: = key): masks by
+//               selection, running maximum (O rescaled in TMEM only when it grows by more than
+//               2^8), exp2, P to TMEM over S's columns (A operand of the next product; thin: to
+//               shared memory, B operand), partials to global memory.
+// S, the sums and O are fp32; P is rounded to the cache's type, as the tensor product takes it,
+// and the sums are over the unrounded P.
+//
+// What bounds it, at 32 query and 8 KV heads of 128 bf16, pages of 64:
+//   prefix (256 requests, 32768 tokens): 141 us, 970 TFLOP/s.  A pair tile takes 4 k cycles, in which
+//     the tensor pipe works 2 k (46 % of the kernel) and the exponential unit 2 k (50 %): each lane's
+//     product -> softmax -> product chain is serial, TMEM holds no third S beside two O of 128
+//     columns, and two lanes cover each other only in part;
+//   own (64 requests, 8192 tokens each): 320 us, 6.7 TB/s, DRAM 83 % busy: HBM;
+//   both (256 requests, 32768 + up to 768): 195 us;
+//   small batches: launches, a prologue of 2.8 us, one tile's latency and the join: 14 us.
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -881,7 +902,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       Job j0{}, j1{};  // pending P V products, j0 the older
       int np = 0;
       uint32_t d = 0, tile = 0, job = 0, nq = 0, pc[2] = {0, 0}, of[2] = {0, 0};
-int in_item = 0;          // key tiles of the item so far
+      int in_item = 0;          // key tiles of the item so far
       int left = 0, rts = 0;    // row tiles of the current key tile still to multiply, of how many
       int flags = 0, vr = 0, stage = 0;
       bool flush = false;
@@ -1577,10 +1598,13 @@ bool prefix_fast_eligible(const PrefixParams& p, int dtype) {
   if (reinterpret_cast<uintptr_t>(p.q) % 16 || reinterpret_cast<uintptr_t>(p.kc) % 16 ||
       reinterpret_cast<uintptr_t>(p.vc) % 16)
     return false;
+  // tensor maps take strides of whole 16 bytes, and no broadcast dimensions
+  const int64_t qn[2] = {p.B, p.H}, kn[3] = {p.num_pages, p.Hkv, p.page};
+  auto loadable = [](int64_t stride, int64_t n) { return stride % 8 == 0 && (stride > 0 || n == 1); };
   for (int i = 0; i < 2; ++i)
-    if (p.qs[i] % 8) return false;
+    if (!loadable(p.qs[i], qn[i])) return false;
   for (int i = 0; i < 3; ++i)
-    if (p.ks[i] % 8 || p.vs[i] % 8) return false;
+    if (!loadable(p.ks[i], kn[i]) || !loadable(p.vs[i], kn[i])) return false;
   return true;
 }
 

@@ -24,6 +24,18 @@ def _workspace_bytes(code, B, H, Hkv, D, page, Lp, L, device_index):
     return max(256, int(nat.lib().sa_ultrametric_prefix_decode_workspace_bytes(code, B, H, Hkv, D, page, Lp, L)))
 
 
+def _rows_load(q: torch.Tensor) -> bool:
+    """Whether q's rows can be loaded where they are: 16-byte aligned, no broadcast dimension.  (Copying
+    a few rows costs a launch; the path that reads any layout takes many times the time.)"""
+    if q.data_ptr() % 16:
+        return False
+    if q.is_contiguous():
+        return True
+    a, b, c = q.stride()
+    unit = 16 // q.element_size()
+    return c == 1 and a > 0 and b > 0 and a % unit == 0 and b % unit == 0
+
+
 def ultrametric_prefix_decode(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -97,7 +109,7 @@ def ultrametric_prefix_decode(
     qri = q_router_indices if q_router_indices.dtype in (i32, i64) else q_router_indices.to(i64)
     kc = k_cache if k_cache.stride(-1) == 1 else k_cache.contiguous()
     vc = v_cache if v_cache.stride(-1) == 1 else v_cache.contiguous()
-    qq = q if q.stride(-1) == 1 else q.contiguous()
+    qq = q if _rows_load(q) else q.clone(memory_format=torch.contiguous_format)
     out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H), dtype=torch.float32, device=q.device) if return_lse else None
     Lp, L, st = pp.shape[0], bt.shape[1], nat.cached_strides

@@ -248,3 +248,30 @@ def test_pool_past_32_bit_offsets():
     got = ultrametric_prefix_decode(d["q"], outs[0], outs[1], d["pp"] + off, n, d["bt"] + off, d["ctx"], ri, d["qri"], 1,
                                     return_lse=True)
     check(t, n, 1, got=got)
+
+
+def test_broadcast_and_unaligned_inputs():
+    t, n = make(5, 8, 2, 128, 16, 130, [0, 5, 33, 17, 64], seed=12)
+    t["q"] = t["q"][:1].expand(5, -1, -1).contiguous()
+    for c in ("kc", "vc"):
+        t[c] = t[c][:, :1].expand(-1, 2, -1, -1).contiguous()
+    d = {k: v.to(DEV) for k, v in t.items()}
+    rest = (d["pp"], n, d["bt"], d["ctx"], d["ri"], d["qri"], 1)
+    heads = [d[c][:, :1].contiguous().expand(-1, 2, -1, -1) for c in ("kc", "vc")]  # one head for both: stride 0
+    qb = d["q"][:1].expand(5, -1, -1)
+    odd = torch.zeros(d["q"].numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view(d["q"].shape)
+    odd.copy_(d["q"])
+    for q, kc, vc in ((qb, d["kc"], d["vc"]), (odd, d["kc"], d["vc"]), (d["q"], *heads), (qb, *heads)):
+        check(t, n, 1, got=ultrametric_prefix_decode(q, kc, vc, *rest, return_lse=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("depth", [0, 1])
+def test_no_own_table_and_no_prefix_list(dtype, depth):
+    t, n = make(19, 8, 2, 64, 16, 210, [0] * 19, dtype=dtype, seed=13)
+    t["bt"] = t["bt"][:, :0].contiguous()
+    check(t, n, depth, 1, True)  # the prefix alone, without a column of own pages
+    t["pp"] = t["pp"][:0].contiguous()
+    check(t, 0, depth, 1, True)  # nothing at all
+    t, _ = make(19, 8, 2, 64, 16, 0, [5 * i for i in range(19)], dtype=dtype, seed=14)
+    check(t, 0, depth)  # own pages alone

@@ -73,51 +73,52 @@ def ultrametric_prefix_decode(
     P, Hkv, page, d2 = k_cache.shape
     if d2 != D or Hkv == 0 or H % Hkv:
         raise ValueError("cache head_dim / heads incompatible with q")
-    if not (q.dtype == k_cache.dtype == v_cache.dtype):
+    dtype = q.dtype
+    if not (k_cache.dtype is dtype and v_cache.dtype is dtype):
         raise ValueError("q, k_cache, v_cache must share dtype")
-    if prefix_pages.dim() != 1 or block_tables.dim() != 2 or block_tables.shape[0] != B or \
-            context_lens.shape != (B,):
+    rows, L = block_tables.shape if block_tables.dim() == 2 else (-1, 0)
+    if rows != B or prefix_pages.dim() != 1 or context_lens.dim() != 1 or context_lens.shape[0] != B:
         raise ValueError(f"expected prefix_pages (Lp,), block_tables ({B}, L) and context_lens ({B},); got "
                          f"{tuple(prefix_pages.shape)}, {tuple(block_tables.shape)}, {tuple(context_lens.shape)}")
-    if router_indices.dim() != 3 or router_indices.shape[:2] != (P, H) or \
-            q_router_indices.dim() != 3 or q_router_indices.shape[:2] != (B, H) or \
-            q_router_indices.shape[2] < 1 or router_indices.shape[2] != q_router_indices.shape[2]:
+    Lp = prefix_pages.shape[0]
+    TD = q_router_indices.shape[2] if q_router_indices.dim() == 3 else 0
+    if TD < 1 or q_router_indices.shape != (B, H, TD) or router_indices.shape != (P, H, TD):
         raise ValueError(f"router_indices must be ({P}, {H}, TD) and q_router_indices ({B}, {H}, TD); got "
                          f"{tuple(router_indices.shape)}, {tuple(q_router_indices.shape)}")
-    TD = q_router_indices.shape[2]
-    if not 0 <= int(req_depth) <= TD:
+    req_depth, local_blocks = int(req_depth), int(local_blocks)
+    if not 0 <= req_depth <= TD:
         raise ValueError(f"req_depth must be in [0, {TD}], got {req_depth}")
-    if int(local_blocks) < 0:
+    if local_blocks < 0:
         raise ValueError(f"local_blocks must be >= 0, got {local_blocks}")
     plen_dev = None
     if isinstance(prefix_len, torch.Tensor):
-        if prefix_len.dtype != torch.int32 or prefix_len.numel() != 1:
+        if prefix_len.dtype is not torch.int32 or prefix_len.numel() != 1:
             raise ValueError(f"prefix_len must be an int or one int32, got {prefix_len.dtype} {tuple(prefix_len.shape)}")
         plen_dev, plen = prefix_len, 0
     else:
         plen = int(prefix_len)
-        if not 0 <= plen <= prefix_pages.shape[0] * page:
-            raise ValueError(f"prefix_len {plen} does not fit {prefix_pages.shape[0]} pages of {page}")
+        if not 0 <= plen <= Lp * page:
+            raise ValueError(f"prefix_len {plen} does not fit {Lp} pages of {page}")
     nat.require_cuda("ultrametric_prefix_decode", q, k_cache, v_cache, prefix_pages, plen_dev, block_tables,
                      context_lens, router_indices, q_router_indices)
-    code = nat.float_code(q.dtype)
+    code = nat.float_code(dtype)
     i32, i64 = torch.int32, torch.int64
     pp = (prefix_pages if prefix_pages.dtype is i32 else prefix_pages.to(i32)).contiguous()
     bt = block_tables if block_tables.dtype is i32 else block_tables.to(i32)
     ctx = (context_lens if context_lens.dtype is i32 else context_lens.to(i32)).contiguous()
     ri = router_indices if router_indices.dtype in (i32, i64) else router_indices.to(i64)
     qri = q_router_indices if q_router_indices.dtype in (i32, i64) else q_router_indices.to(i64)
-    kc = k_cache if k_cache.stride(-1) == 1 else k_cache.contiguous()
-    vc = v_cache if v_cache.stride(-1) == 1 else v_cache.contiguous()
+    kc = k_cache if k_cache.stride()[3] == 1 else k_cache.contiguous()
+    vc = v_cache if v_cache.stride()[3] == 1 else v_cache.contiguous()
     qq = q if _rows_load(q) else q.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H), dtype=torch.float32, device=q.device) if return_lse else None
-    Lp, L, st = pp.shape[0], bt.shape[1], nat.cached_strides
+    out = torch.empty_like(qq, memory_format=torch.contiguous_format)
+    lse = q.new_empty((B, H), dtype=torch.float32) if return_lse else None
     ws_bytes = _workspace_bytes(code, B, H, Hkv, D, page, Lp, L, q.get_device())
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
+    st, ptr = nat.cached_strides, nat.ptr
     nat.check(nat.lib().sa_ultrametric_prefix_decode(
         code, B, H, Hkv, D, page, P, qq.data_ptr(), st(qq), kc.data_ptr(), st(kc), vc.data_ptr(), st(vc), pp.data_ptr(), Lp,
-        plen, nat.ptr(plen_dev), bt.data_ptr(), st(bt), L, ctx.data_ptr(), ri.data_ptr(), nat.int_code(ri.dtype), st(ri),
-        qri.data_ptr(), nat.int_code(qri.dtype), st(qri), TD, int(req_depth), int(local_blocks), int(bool(sink_block)),
-        out.data_ptr(), st(out), nat.ptr(lse), ws.data_ptr(), ws_bytes, nat.raw_stream(q)), "ultrametric_prefix_decode")
+        plen, ptr(plen_dev), bt.data_ptr(), st(bt), L, ctx.data_ptr(), ri.data_ptr(), nat.int_code(ri.dtype), st(ri),
+        qri.data_ptr(), nat.int_code(qri.dtype), st(qri), TD, req_depth, local_blocks, int(bool(sink_block)),
+        out.data_ptr(), st(out), ptr(lse), ws.data_ptr(), ws_bytes, nat.raw_stream(q)), "ultrametric_prefix_decode")
     return (out, lse) if return_lse else out

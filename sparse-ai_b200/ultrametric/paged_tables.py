@@ -44,25 +44,24 @@ class PagedTables(NamedTuple):
     num_free: torch.Tensor
 
 
-def _int32(name: str, t: torch.Tensor, shape: tuple) -> torch.Tensor:
-    if t.dtype is not torch.int32 or t.shape != shape:
-        raise ValueError(f"{name} must be int32 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    return t
-
-
-def _tables_args(context_lens, block_tables, free_pages, num_free, page_size):
+def _tables_args(context_lens, block_tables, free_pages, num_free, page_size, per_request):
+    """(B, L) of checked arguments; ``per_request`` = (name, tensor, dtype) beside the lengths."""
+    i32 = torch.int32
     if context_lens.dim() != 1 or block_tables.dim() != 2 or free_pages.dim() != 1:
         raise ValueError("context_lens and free_pages must be 1-d and block_tables 2-d; got "
                          f"{tuple(context_lens.shape)}, {tuple(free_pages.shape)}, {tuple(block_tables.shape)}")
-    B, L = context_lens.shape[0], block_tables.shape[1]
-    _int32("context_lens", context_lens, (B,))
-    _int32("block_tables", block_tables, (B, L))
-    _int32("free_pages", free_pages, (free_pages.shape[0],))
-    if num_free.dtype != torch.int32 or num_free.numel() != 1:
+    (B,), (rows, L) = shape, _ = context_lens.shape, block_tables.shape
+    name, t, dtype = per_request
+    if not (context_lens.dtype is i32 and block_tables.dtype is i32 and free_pages.dtype is i32) or rows != B:
+        raise ValueError(f"context_lens, block_tables and free_pages must be int32 of shapes ({B},), ({B}, L) and (F,); got "
+                         + ", ".join(f"{x.dtype} {tuple(x.shape)}" for x in (context_lens, block_tables, free_pages)))
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} of shape ({B},), got {t.dtype} {tuple(t.shape)}")
+    if num_free.dtype is not i32 or num_free.numel() != 1:
         raise ValueError(f"num_free must be one int32, got {num_free.dtype} {tuple(num_free.shape)}")
     if not free_pages.is_contiguous():
         raise ValueError("free_pages must be contiguous")
-    if int(page_size) < 1:
+    if page_size < 1:
         raise ValueError(f"page_size must be >= 1, got {page_size}")
     return B, L
 
@@ -93,27 +92,27 @@ def build_paged_tables(
     no pages left) is refused: its rows get slot -1, its length and table stay, and the device
     status gets bit 2.  Requests after one that found no pages are refused too if they need any.
     Nothing is read back to the host."""
-    B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size)
-    _int32("new_lens", new_lens, (B,))
-    if int(num_tokens) < 0:
+    page_size, T, position_base = int(page_size), int(num_tokens), int(position_base)
+    B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size,
+                        ("new_lens", new_lens, torch.int32))
+    if T < 0:
         raise ValueError(f"num_tokens must be >= 0, got {num_tokens}")
-    if int(position_base) < 0:
+    if position_base < 0:
         raise ValueError(f"position_base must be >= 0, got {position_base}")
     nat.require_cuda("build_paged_tables", context_lens, new_lens, block_tables, free_pages, num_free)
-    dev, T = context_lens.device, int(num_tokens)
     ctx, new = context_lens.contiguous(), new_lens.contiguous()
-    slots = torch.empty(T, dtype=torch.int64, device=dev)
-    # the int32 results share one allocation, each on a 16-byte boundary
-    Tp, Bp = (T + 3) & ~3, (B + 4) & ~3
-    buf = torch.empty(2 * Tp + 2 * Bp + 4, dtype=torch.int32, device=dev)
-    rid, pos, cu, ctx_out, free_out = buf.as_strided((T,), (1,), 0), buf.as_strided((T,), (1,), Tp), \
-        buf.as_strided((B + 1,), (1,), 2 * Tp), buf.as_strided((B,), (1,), 2 * Tp + Bp), buf.as_strided((1,), (1,), 2 * Tp + 2 * Bp)
+    slots = ctx.new_empty(T, dtype=torch.int64)
+    # the int32 results share one allocation, those by token on 16-byte boundaries
+    pad = -T % 4
+    buf = ctx.new_empty(2 * (T + pad) + 2 * B + 2)
+    rid, _, pos, _, cu, ctx_out, free_out = buf.unsafe_split_with_sizes((T, pad, T, pad, B + 1, B, 1))
     p0 = buf.data_ptr()
+    p1 = p0 + 8 * (T + pad)
     nat.check(nat.lib().sa_paged_build_tables(
-        B, L, int(page_size), T, ctx.data_ptr(), new.data_ptr(), block_tables.data_ptr(),
+        B, L, page_size, T, ctx.data_ptr(), new.data_ptr(), block_tables.data_ptr(),
         nat.cached_strides(block_tables), free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(),
-        int(position_base), slots.data_ptr(), p0, p0 + 4 * Tp, p0 + 8 * Tp, p0 + 4 * (2 * Tp + Bp),
-        p0 + 8 * (Tp + Bp), nat.raw_stream(ctx)), "build_paged_tables")
+        position_base, slots.data_ptr(), p0, p0 + 4 * (T + pad), p1, p1 + 4 * (B + 1), p1 + 4 * (2 * B + 1),
+        nat.raw_stream(ctx)), "build_paged_tables")
     return PagedTables(slots, rid, pos, cu, ctx_out, free_out)
 
 
@@ -129,14 +128,14 @@ def release_paged_requests(
     """Push the pages of every request with ``finished[b]`` ((B,) bool) back on the stack, in
     request order; returns the new (context_lens, num_free).  ``free_pages`` is written above its
     old height; the block tables are left as they are."""
-    B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size)
-    if finished.dtype != torch.bool or tuple(finished.shape) != (B,):
-        raise ValueError(f"finished must be bool of shape {(B,)}, got {finished.dtype} {tuple(finished.shape)}")
+    page_size = int(page_size)
+    B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size,
+                        ("finished", finished, torch.bool))
     nat.require_cuda("release_paged_requests", finished, context_lens, block_tables, free_pages, num_free)
     ctx, done = context_lens.contiguous(), finished.contiguous()
-    out_ctx, out_free = torch.empty_like(ctx), torch.empty(1, dtype=torch.int32, device=ctx.device)
+    out_ctx, out_free = torch.empty_like(ctx), ctx.new_empty(1)
     nat.check(nat.lib().sa_paged_release(
-        B, L, int(page_size), done.data_ptr(), ctx.data_ptr(), block_tables.data_ptr(), nat.cached_strides(block_tables),
+        B, L, page_size, done.data_ptr(), ctx.data_ptr(), block_tables.data_ptr(), nat.cached_strides(block_tables),
         free_pages.data_ptr(), free_pages.shape[0], num_free.data_ptr(), out_ctx.data_ptr(), out_free.data_ptr(),
         nat.raw_stream(ctx)), "release_paged_requests")
     return out_ctx, out_free
@@ -163,29 +162,31 @@ def paged_kv_write(
     if k.dim() != 3 or v.shape != k.shape:
         raise ValueError(f"k and v must be (T, Hkv, D); got {tuple(k.shape)}, {tuple(v.shape)}")
     T, Hkv, D = k.shape
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+    P, h2, page, d2 = k_cache.shape if k_cache.dim() == 4 else (0, -1, 0, -1)
+    if h2 != Hkv or d2 != D or v_cache.shape != k_cache.shape:
         raise ValueError(f"k_cache/v_cache must be (num_pages, {Hkv}, page_size, {D}); got "
                          f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+    dtype = k.dtype
+    if not (v.dtype is dtype and k_cache.dtype is dtype and v_cache.dtype is dtype):
         raise ValueError("k, v, k_cache, v_cache must share dtype")
-    if slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (T,):
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or slot_mapping.shape[0] != T:
         raise ValueError(f"slot_mapping must be int64 of shape {(T,)}, got {slot_mapping.dtype} "
                          f"{tuple(slot_mapping.shape)}")
     if (routes is None) != (router_indices is None):
         raise ValueError("routes and router_indices go together")
     H = TD = 0
     if routes is not None:
-        if routes.dim() != 3 or router_indices.dim() != 3 or routes.shape[0] != T or \
-                router_indices.shape[0] != k_cache.shape[0] or routes.shape[1:] != router_indices.shape[1:]:
+        t2, H, TD = routes.shape if routes.dim() == 3 else (-1, 0, 0)
+        if t2 != T or router_indices.shape != (P, H, TD):
             raise ValueError(f"routes must be (T, H, TD) and router_indices (num_pages, H, TD); got "
                              f"{tuple(routes.shape)}, {tuple(router_indices.shape)}")
-        H, TD = routes.shape[1:]
-    if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
+    kst, vst, kcs, vcs = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    if kcs[3] != 1 or vcs[3] != 1:
         raise ValueError("the caches' head_dim must be contiguous")
     nat.require_cuda("paged_kv_write", k, v, slot_mapping, k_cache, v_cache, routes, router_indices)
-    code = nat.float_code(k.dtype)
-    kk = k if k.stride(-1) == 1 else k.contiguous()
-    vv = v if v.stride(-1) == 1 else v.contiguous()
+    code = nat.float_code(dtype)
+    kk = k if kst[2] == 1 else k.contiguous()
+    vv = v if vst[2] == 1 else v.contiguous()
     slots = slot_mapping.contiguous()
     st = nat.cached_strides
     if routes is None:
@@ -194,6 +195,5 @@ def paged_kv_write(
         r_args = (routes.data_ptr(), nat.int_code(routes.dtype), st(routes), H, TD, router_indices.data_ptr(),
                   nat.int_code(router_indices.dtype), st(router_indices))
     nat.check(nat.lib().sa_paged_kv_write(
-        code, T, Hkv, D, k_cache.shape[2], k_cache.shape[0], kk.data_ptr(), st(kk), vv.data_ptr(), st(vv),
-        slots.data_ptr(), k_cache.data_ptr(), st(k_cache), v_cache.data_ptr(), st(v_cache), *r_args,
-        nat.raw_stream(k_cache)), "paged_kv_write")
+        code, T, Hkv, D, page, P, kk.data_ptr(), st(kk), vv.data_ptr(), st(vv), slots.data_ptr(), k_cache.data_ptr(),
+        st(k_cache), v_cache.data_ptr(), st(v_cache), *r_args, nat.raw_stream(k_cache)), "paged_kv_write")

@@ -13,6 +13,7 @@ namespace sa {
 namespace {
 
 constexpr int kWriteThreads = 256;
+constexpr int kMaxGroups = 16;
 
 struct WriteParams {
   const char* kn;
@@ -29,40 +30,50 @@ struct WriteParams {
   int router_dtype;
   int64_t rrs[3];
   int64_t T, Hkv, row_bytes, page, num_pages, H, TD;
+  int groups;  // token groups side by side in a CTA
   unsigned* status;
 };
 
-// A CTA copies kTok consecutive tokens; V is the unit of the copies (16, 8, 4 or 2 bytes: the
-// widest that every address and stride allows).  A thread keeps its place within the row (K or V,
-// head, unit) and takes that unit of all the CTA's tokens: the loads, which need no slot, are all in
-// flight while the slots arrive and are divided into page and row, once per token.
+// A CTA copies groups * kTok consecutive tokens; V is the unit of the copies (16, 8, 4 or 2 bytes: the
+// widest that every address and stride allows).  A token takes 2 Hkv row_bytes / sizeof(V) threads
+// (at most all of them, in turns); where that is a half or less of the CTA, `groups` of them work
+// side by side on neighbouring tokens.  A thread keeps its place within the row (K or V, head, unit)
+// and takes that unit of its kTok tokens: the loads, which need no slot, are all in flight while
+// the slots arrive and are divided into page and row, once per token.
 //
 // Bound by HBM: 2 T Hkv D elements in and as many out.  32768 tokens of 8 heads of 128 bf16 (268 MB
-// of traffic): one token per CTA 95 us, 8 tokens 48 us (5.6 TB/s; a plain copy runs at 6.5).  Below
+// of traffic): one token per CTA 95 us, 8 tokens 46 us (5.9 TB/s; a plain copy runs at 6.5).  Below
 // about 8 tokens per SM the CTAs would not cover the GPU, and one token per CTA ends sooner.
+// 32768 tokens of 2 heads of 64 bf16 (32 threads a token): one group 14.3 us, 8 groups 10.0.
 template <typename V, int kTok>
 __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteParams p) {
-  __shared__ int64_t s_page[kTok], s_row[kTok];  // page -1: no slot
-  const int64_t t0 = (int64_t)blockIdx.x * kTok;
+  __shared__ int64_t s_page[kTok * kMaxGroups], s_row[kTok * kMaxGroups];  // page -1: no slot
+  const int groups = p.groups, tokens = kTok * groups;
+  const int64_t t0 = (int64_t)blockIdx.x * tokens;
   const int tid = threadIdx.x;
   const int per_head = (int)(p.row_bytes / sizeof(V)), units = per_head * (int)p.Hkv;
-  int u = tid;
+  int u = tid, g = 0;
+  if (groups > 1) {
+    g = tid / (2 * units);
+    u = g < groups ? tid - g * 2 * units : 2 * units;
+  }
   V x[kTok];
   bool is_v = false;
   int h = 0, c = 0;
-  auto load = [&]() {  // unit u of every token
+  auto load = [&]() {  // unit u of tokens g, g + groups, ...
     is_v = u >= units;
     const int uu = is_v ? u - units : u;
     h = uu / per_head;
     c = uu - h * per_head;
     const int64_t* ns = is_v ? p.vns : p.kns;
-    const char* src = (is_v ? p.vn : p.kn) + t0 * ns[0] + h * ns[1] + (int64_t)c * (int)sizeof(V);
+    const char* src = (is_v ? p.vn : p.kn) + (t0 + g) * ns[0] + h * ns[1] + (int64_t)c * (int)sizeof(V);
+    const int64_t step = groups * ns[0];
 #pragma unroll
     for (int j = 0; j < kTok; ++j)
-      if (t0 + j < p.T) x[j] = *reinterpret_cast<const V*>(src + j * ns[0]);
+      if (t0 + g + j * groups < p.T) x[j] = *reinterpret_cast<const V*>(src + j * step);
   };
   if (u < 2 * units) load();
-  if (tid < kTok) {
+  if (tid < tokens) {
     const int64_t slot = t0 + tid < p.T ? p.slots[t0 + tid] : -1;
     int64_t page = slot < 0 ? -1 : slot / p.page;
     s_row[tid] = slot - page * p.page;
@@ -77,31 +88,42 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteP
     const int64_t* cs = is_v ? p.vs : p.ks;
     char* dst = (is_v ? p.vc : p.kc) + h * cs[1] + (int64_t)c * (int)sizeof(V);
 #pragma unroll
-    for (int j = 0; j < kTok; ++j)
-      if (s_page[j] >= 0) *reinterpret_cast<V*>(dst + s_page[j] * cs[0] + s_row[j] * cs[2]) = x[j];
+    for (int j = 0; j < kTok; ++j) {
+      const int i = g + j * groups;
+      if (s_page[i] >= 0) *reinterpret_cast<V*>(dst + s_page[i] * cs[0] + s_row[i] * cs[2]) = x[j];
+    }
     u += kWriteThreads;
     if (u < 2 * units) load();
   }
   if (!p.routes) return;
   // Routing vectors, one warp per token: a page takes that of the last of its rows, i.e. of a row whose
-  // next row with a slot is in another page (rows without one are passed over, 32 at a time).
+  // next row with a slot is in another page.  Rows without one are passed over: 32 at first, then 512
+  // at a time (a batch padded to a fixed size ends in thousands of them).
   const int lane = tid & 31;
-  constexpr bool kAll = kTok == 1;  // the CTA's warps share its only token
-  for (int j = kAll ? 0 : tid >> 5; j < kTok; j += kAll ? 1 : kWriteThreads / 32) {
+  const bool all = tokens == 1;  // the CTA's warps share its only token
+  for (int j = all ? 0 : tid >> 5; j < tokens; j += all ? 1 : kWriteThreads / 32) {
     const int64_t t = t0 + j, page = s_page[j];
     if (page < 0) continue;
-    bool last = true;
-    for (int64_t n0 = t + 1; n0 < p.T; n0 += 32) {
-      const int64_t next = n0 + lane < p.T ? p.slots[n0 + lane] : -1;
-      const unsigned has = __ballot_sync(0xffffffffu, next >= 0);
-      if (!has) continue;
-      const int64_t first = __shfl_sync(0xffffffffu, next, __ffs(has) - 1);
-      last = first < page * p.page || first >= (page + 1) * p.page;
-      break;
+    int64_t n0 = t + 1, first = -1;  // the next slot
+    int64_t next = n0 + lane < p.T ? p.slots[n0 + lane] : -1;
+    unsigned has = __ballot_sync(0xffffffffu, next >= 0);
+    if (has) first = __shfl_sync(0xffffffffu, next, __ffs(has) - 1);
+#pragma unroll 1
+    for (n0 += 32; !has && n0 < p.T; n0 += 32 * 16) {
+      unsigned found = 0;  // bit k: row n0 + 32 k + lane has a slot
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        found |= n0 + 32 * k + lane < p.T && p.slots[n0 + 32 * k + lane] >= 0 ? 1u << k : 0u;
+      const unsigned any = __reduce_or_sync(0xffffffffu, found);
+      if (!any) continue;
+      const int k = __ffs(any) - 1;
+      has = __ballot_sync(0xffffffffu, (found >> k) & 1u);
+      first = p.slots[n0 + 32 * k + __ffs(has) - 1];
     }
+    const bool last = !has || first < page * p.page || first >= (page + 1) * p.page;
     if (!last) continue;
     const int n = (int)(p.H * p.TD), TD = (int)p.TD;
-    for (int i = kAll ? tid : lane; i < n; i += kAll ? kWriteThreads : 32) {
+    for (int i = all ? tid : lane; i < n; i += all ? kWriteThreads : 32) {
       const int hh = i / TD, l = i - hh * TD;
       const int64_t v = load_any_i64(p.routes, p.routes_dtype, t * p.rts[0] + hh * p.rts[1] + l * p.rts[2]);
       const int64_t o = page * p.rrs[0] + hh * p.rrs[1] + l * p.rrs[2];
@@ -113,15 +135,22 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteP
   }
 }
 
-// Tokens per CTA: kWide where that still gives every SM a CTA, else 1.
+// Tokens per thread: kWide where that still gives every SM a CTA, else 1.
 constexpr int kWide = 8;
 
 template <typename V>
-void launch_write(const WriteParams& p, cudaStream_t s) {
-  if (p.T >= (int64_t)kWide * device_sm_count())
-    paged_write_kernel<V, kWide><<<(unsigned)((p.T + kWide - 1) / kWide), kWriteThreads, 0, s>>>(p);
+void launch_write(WriteParams p, cudaStream_t s) {
+  const int64_t threads = 2 * p.Hkv * (p.row_bytes / (int64_t)sizeof(V)), sms = device_sm_count();
+  // as many groups as fit, but not so many that there are fewer than two CTAs per SM (3001 tokens of
+  // 120 threads: one group 3.2 us, two 3.6)
+  p.groups = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxGroups, kWriteThreads / threads, p.T / (2 * kWide * sms)}));
+  const bool wide = p.T >= kWide * sms;
+  const int64_t tokens = p.groups * (wide ? kWide : 1);
+  const unsigned grid = (unsigned)((p.T + tokens - 1) / tokens);
+  if (wide)
+    paged_write_kernel<V, kWide><<<grid, kWriteThreads, 0, s>>>(p);
   else
-    paged_write_kernel<V, 1><<<(unsigned)p.T, kWriteThreads, 0, s>>>(p);
+    paged_write_kernel<V, 1><<<grid, kWriteThreads, 0, s>>>(p);
 }
 
 }  // namespace

@@ -183,3 +183,24 @@ def test_write_past_32_bit_offsets():
     paged_kv_write(k, k, slots, kc, kc)
     assert torch.equal(kc[P - 1, :, page - 1], k[0]) and torch.equal(kc[P - 9, :, 3], k[1])
     assert nat.read_device_status(reset=True) == 0
+
+
+@pytest.mark.parametrize("T,live,Hkv,D,dtype", [(5000, 4700, 1, 64, torch.bfloat16), (9000, 40, 2, 80, torch.float32),
+                                                (2400, 2399, 3, 20, torch.float16), (700, 1, 1, 8, torch.float32)])
+def test_write_small_rows_with_gaps_and_padding(T, live, Hkv, D, dtype):
+    torch.manual_seed(T)
+    page, H, TD = 16, 4, 2
+    P = -(-T // page) + 3
+    slots = torch.randperm((P - 1) * page, device=DEV)[:T].sort().values
+    slots[torch.rand(T, device=DEV) < 0.2] = -1
+    slots[live - 1] = slots.max() + 1
+    slots[live:] = -1
+    k, v = _randn((T, Hkv, D), dtype), _randn((T, Hkv, D), dtype)
+    kc, vc = torch.zeros(P, Hkv, page, D, dtype=dtype, device=DEV), torch.zeros(P, Hkv, page, D, dtype=dtype, device=DEV)
+    routes = torch.randint(0, 9, (T, H, TD), device=DEV, dtype=torch.int32)
+    router = torch.full((P, H, TD), -1, dtype=torch.int32, device=DEV)
+    want = [x.cpu().clone() for x in (kc, vc, router)]
+    so.write_rows(k.cpu(), v.cpu(), slots.cpu(), want[0], want[1], routes.cpu(), want[2])
+    paged_kv_write(k, v, slots, kc, vc, routes=routes, router_indices=router)
+    assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1]) and torch.equal(router.cpu(), want[2])
+    assert nat.read_device_status(reset=True) == 0

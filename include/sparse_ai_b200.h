@@ -414,8 +414,9 @@ SA_API int64_t sa_ultrametric_prefix_decode_workspace_bytes(int dtype, int64_t B
  * one of the last local_blocks.  Lengths are cut to their page lists; pages outside [0, num_pages)
  * are skipped (status bit 2).  A row with nothing to attend gets zeros and lse = -inf.
  *
- * dtype             SA_BF16, SA_F16 (tcgen05 path where D % 8 == 0, D <= 128, page_size % 8 == 0
- *                   and every row of q and the caches is 16-byte aligned) or SA_F32; D <= 256.
+ * dtype             SA_BF16, SA_F16 (tcgen05 path where D % 8 == 0, D <= 128, page_size % 8 == 0,
+ *                   H / Hkv <= 128, H <= 256, and every row of q and the caches is 16-byte aligned
+ *                   with no stride of 0) or SA_F32; D <= 256.
  * q, out            (B, H, D); k_cache, v_cache (P, Hkv, page_size, D); D contiguous.
  * prefix_pages      (max_prefix_pages,) int32; block_tables (B, max_logical_pages) int32.
  * router            (P, H, TD), q_router (B, H, TD): SA_I32 or SA_I64 (not read at req_depth 0).

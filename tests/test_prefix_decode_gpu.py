@@ -275,3 +275,19 @@ def test_no_own_table_and_no_prefix_list(dtype, depth):
     check(t, 0, depth, 1, True)  # nothing at all
     t, _ = make(19, 8, 2, 64, 16, 0, [5 * i for i in range(19)], dtype=dtype, seed=14)
     check(t, 0, depth)  # own pages alone
+
+
+@pytest.mark.parametrize("B,H,Hkv,D,page,prefix,hi", [
+    (60, 9, 3, 64, 16, 300, 40),    # groups of 3: 126 of a tile's 128 rows
+    (41, 35, 5, 128, 32, 700, 70),  # 7
+    (9, 34, 2, 96, 64, 260, 200),   # 17: own items in the 128-row form
+    (5, 132, 2, 64, 16, 333, 90),   # 66: one request per row tile
+    (3, 128, 1, 128, 64, 500, 130),
+    (17, 256, 16, 64, 128, 900, 300),
+    (300, 4, 4, 128, 64, 128, 3),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("depth", [0, 1])
+def test_group_sizes(B, H, Hkv, D, page, prefix, hi, dtype, depth):
+    t, n = make(B, H, Hkv, D, page, prefix, [(i * 37 + 5) % (hi + 1) for i in range(B)], dtype=dtype, seed=B)
+    check(t, n, depth, depth, bool(depth))

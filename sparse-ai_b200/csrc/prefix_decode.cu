@@ -15,7 +15,10 @@
 // stride and element type; fp32 arithmetic on the CUDA cores).  A CTA takes up to kRows rows of one
 // KV head and a range of 32-key tiles: K and V of a tile go to shared memory once and serve all
 // its rows, as float4s: 16 products per 5 loads.  Batches that need it are small (a 32-bit cache, odd
-// sizes), so it is bound by latency along its few tiles.
+// sizes), so it is bound by latency: the round trips to memory one after the other (page, routes, Q, K,
+// V, parts), of which each has all its loads in flight.  5 requests, 12 heads of 80 fp32, 1000 + up to
+// 100 tokens: 20.6 us (34.3 with loads in short loops and the join as an ordinary launch).  Large
+// batches are bound by shared memory: 8 requests of 64 / 8 heads of 128 fp32 on 2000 tokens, 71 us.
 #include <algorithm>
 #include <string>
 
@@ -37,7 +40,7 @@ struct PdSplit {
 };
 
 // Splits so that both kinds of work reach about four CTAs per SM, down to one key tile each over the
-// lists' widths (the lengths are on the device): a tile takes a CTA about 10 us, all latency.
+// lists' widths (the lengths are on the device): a tile takes a CTA about 5 us, all latency.
 PdSplit pd_split(int64_t B, int64_t H, int64_t Hkv, int64_t page, int64_t Lp, int64_t L) {
   PdSplit s;
   const int64_t G = H / Hkv;
@@ -60,7 +63,7 @@ int64_t pd_bytes(int64_t B, int64_t H, int64_t D, const PdSplit& s) {
 
 // NI: float4 output columns per thread, D <= 32 NI.
 template <typename T, int NI>
-__global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixParams p, const PdSplit s, float* part) {
+__global__ void __launch_bounds__(kPdThreads, NI <= 4 ? 5 : 3) prefix_split_kernel(const PrefixParams p, const PdSplit s, float* part) {
   extern __shared__ float sm[];
   // rows of D floats, padded with zeros to whole float4s and by one more, so that the eight keys that
   // a row's threads read at a time lie in different banks
@@ -73,6 +76,7 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
   __shared__ int s_phys[kKeys], s_lp[kKeys];
   __shared__ const T *s_krow[kKeys], *s_vrow[kKeys];
   const int tid = threadIdx.x;
+  pdl_trigger();  // the join waits for the whole grid
 
   // ---- which rows and which keys
   const int64_t prefix_ctas = p.Hkv * s.row_tiles * s.sp;
@@ -113,10 +117,22 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
   const float scale2 = rsqrtf((float)D) * kLog2e;
   {
     const int warp = tid >> 5, lane = tid & 31;
-    for (int rr = warp; rr < kRows; rr += kPdThreads / 32) {
-      const int rg = (int)row0 + rr, bb = rg / (int)p.G, hh = (int)g * (int)p.G + rg - bb * (int)p.G;
-      const T* q = static_cast<const T*>(p.q) + bb * p.qs[0] + hh * p.qs[1];
-      for (int d = lane; d < 4 * D4; d += 32) s_q[rr * DP + d] = rr < nrows && d < D ? to_f32<T>(q[d]) * scale2 : 0.f;
+    constexpr int kPer = kRows / (kPdThreads / 32);
+    const T* q[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int rg = (int)min(row0 + warp + u * (kPdThreads / 32), p.B * p.G - 1), bb = rg / (int)p.G;
+      q[u] = static_cast<const T*>(p.q) + bb * p.qs[0] + (g * p.G + rg - bb * p.G) * p.qs[1];
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int d = lane + 32 * i;
+      float x[kPer];
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) x[u] = d < D ? to_f32<T>(q[u][d]) * scale2 : 0.f;
+#pragma unroll
+      for (int u = 0; u < kPer; ++u)
+        if (d < 4 * D4) s_q[(warp + u * (kPdThreads / 32)) * DP + d] = x[u];
     }
   }
   float m = -INFINITY, l = 0.f;
@@ -164,13 +180,30 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
     if (!__syncthreads_or(any)) continue;
     // one warp per key, lanes along the row; all of a warp's loads in flight
     const int warp = tid >> 5, lane = tid & 31;
-    for (int d = lane; d < 4 * D4; d += 32) {
+    constexpr int kPer = kKeys / (kPdThreads / 32), kRound = NI < 4 ? NI : 4;
 #pragma unroll
-      for (int u = 0; u < kKeys / (kPdThreads / 32); ++u) {
-        const int kk = warp + u * (kPdThreads / 32);
-        const bool have = s_phys[kk] >= 0 && d < D;
-        s_k[kk * DP + d] = have ? to_f32<T>(s_krow[kk][d]) : 0.f;
-        s_v[kk * DP + d] = have ? to_f32<T>(s_vrow[kk][d]) : 0.f;
+    for (int i0 = 0; i0 < NI; i0 += kRound) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        float x[kRound][kPer];
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+          const int kk = warp + u * (kPdThreads / 32);
+          const bool have = s_phys[kk] >= 0;
+          const T* src = kv ? s_vrow[kk] : s_krow[kk];
+#pragma unroll
+          for (int i = 0; i < kRound; ++i) {
+            const int d = lane + 32 * (i0 + i);
+            x[i][u] = have && d < D ? to_f32<T>(src[d]) : 0.f;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kPer; ++u)
+#pragma unroll
+          for (int i = 0; i < kRound; ++i) {
+            const int d = lane + 32 * (i0 + i);
+            if (d < 4 * D4) (kv ? s_v : s_k)[(warp + u * (kPdThreads / 32)) * DP + d] = x[i][u];
+          }
       }
     }
     __syncthreads();
@@ -246,42 +279,77 @@ __global__ void __launch_bounds__(kPdThreads) prefix_split_kernel(const PrefixPa
   }
 }
 
-// Joins the parts of (b, h) = blockIdx.x.
+// Joins the parts of (b, h) = blockIdx.x.  Two dependent rounds of loads (the parts' m and l, then their
+// accumulators): warps share the parts, lanes the columns, 16 loads in flight each.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+
 template <typename T>
-__global__ void __launch_bounds__(kPdThreads) prefix_join_kernel(const PrefixParams p, const PdSplit s,
-                                                                 const float* part) {
+__global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const PrefixParams p, const PdSplit s,
+                                                                   const float* part) {
   const int64_t b = blockIdx.x / p.H, h = blockIdx.x % p.H;
-  const int n = s.sp + s.so, D = (int)p.D, tid = threadIdx.x;
+  const int n = s.sp + s.so, D = (int)p.D, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float* base = part + (int64_t)blockIdx.x * n * (D + 2);
-  __shared__ float s_m[2 * kMaxSplits], s_w[2 * kMaxSplits];
-  __shared__ float s_l[2 * kMaxSplits];
-  if (tid < n) {  // n <= 2 kMaxSplits == kPdThreads
-    s_m[tid] = base[(int64_t)tid * (D + 2)];
-    s_l[tid] = base[(int64_t)tid * (D + 2) + 1];
+  __shared__ float s_m[2 * kMaxSplits], s_l[2 * kMaxSplits], s_w[2 * kMaxSplits];
+  __shared__ float s_a[kJoinWarps][128];
+  pdl_wait();
+  if (tid < 2 * kMaxSplits) {
+    s_m[tid] = tid < n ? base[(int64_t)tid * (D + 2)] : -INFINITY;
+    s_l[tid] = tid < n ? base[(int64_t)tid * (D + 2) + 1] : 0.f;
   }
   __syncthreads();
   float M = -INFINITY;
-  for (int i = 0; i < n; ++i) M = fmaxf(M, s_m[i]);
+#pragma unroll
+  for (int k = 0; k < 2 * kMaxSplits; k += 32) M = fmaxf(M, s_m[k + lane]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   const float ref = M == -INFINITY ? 0.f : M;
-  if (tid < n) s_w[tid] = exp2f(s_m[tid] - ref);
-  __syncthreads();
   float L = 0.f;
-  for (int i = 0; i < n; ++i) L += s_l[i] * s_w[i];
+#pragma unroll
+  for (int k = 0; k < 2 * kMaxSplits; k += 32) {
+    const float w = exp2f(s_m[k + lane] - ref);
+    if (warp == 0) s_w[k + lane] = w;
+    L += s_l[k + lane] * w;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  __syncthreads();
   const float inv = L == 0.f ? 0.f : 1.f / L;  // NaN stays NaN
   T* o = static_cast<T*>(p.out) + b * p.os[0] + h * p.os[1];
-  for (int d = tid; d < D; d += kPdThreads) {
-    float a = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float x = base[(int64_t)i * (D + 2) + 2 + d];
-      if (s_m[i] != -INFINITY) a = fmaf(x, s_w[i], a);
+  for (int d0 = 0; d0 < D; d0 += 128) {
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int i0 = warp; i0 < n; i0 += 4 * kJoinWarps) {
+      float x[4][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i0 + u * kJoinWarps, d = d0 + 32 * k + lane;
+          x[u][k] = i < n && d < D ? base[(int64_t)i * (D + 2) + 2 + d] : 0.f;
+        }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kJoinWarps;
+        if (i < n && s_m[i] != -INFINITY)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) a[k] = fmaf(x[u][k], s_w[i], a[k]);
+      }
     }
-    o[d] = from_f32<T>(L == 0.f ? 0.f : a * inv);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s_a[warp][32 * k + lane] = a[k];
+    __syncthreads();
+    if (tid < 128 && d0 + tid < D) {
+      float y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) y += s_a[w][tid];
+      o[d0 + tid] = from_f32<T>(L == 0.f ? 0.f : y * inv);
+    }
+    __syncthreads();
   }
   if (p.lse && tid == 0) p.lse[blockIdx.x] = L == 0.f ? -INFINITY : M * kLn2 + logf(L);
 }
 
-static_assert(2 * kMaxSplits == kPdThreads, "one thread per part in the join");
+static_assert(2 * kMaxSplits == 128, "whole warps of parts in the join");
 
 template <typename T>
 int launch_general(const PrefixParams& p, float* part, cudaStream_t stream) {
@@ -297,8 +365,8 @@ int launch_general(const PrefixParams& p, float* part, cudaStream_t stream) {
     kern<<<(unsigned)ctas, kPdThreads, smem, stream>>>(p, s, part);
     if (int rc = check_launch("prefix_split_kernel")) return rc;
   }
-  prefix_join_kernel<T><<<(unsigned)(p.B * p.H), kPdThreads, 0, stream>>>(p, s, part);
-  return check_launch("prefix_join_kernel");
+  return launch_dependent(prefix_join_kernel<T>, dim3((unsigned)(p.B * p.H)), dim3(kJoinThreads), 0, stream,
+                          "prefix_join_kernel", p, s, (const float*)part);
 }
 
 }  // namespace

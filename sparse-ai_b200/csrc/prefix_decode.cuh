@@ -48,10 +48,16 @@ __device__ __forceinline__ int64_t own_tokens(const PrefixParams& p, int64_t b) 
 __device__ __forceinline__ bool page_attended(const PrefixParams& p, int64_t b, int64_t h, int64_t l, int64_t n,
                                               int64_t phys) {
   if ((p.sink && l == 0) || l >= n - p.local_blocks) return true;
-  for (int64_t i = 0; i < p.r; ++i)
-    if (load_any_i64(p.router, p.router_dtype, phys * p.rs[0] + h * p.rs[1] + i * p.rs[2]) !=
-        load_any_i64(p.qrouter, p.qrouter_dtype, b * p.qrs[0] + h * p.qrs[1] + i * p.qrs[2]))
-      return false;
+  for (int64_t i = 0; i < p.r; i += 4) {  // 4 levels in flight; those past r repeat the last
+    bool same = true;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t lv = min(i + k, p.r - 1);
+      same &= load_any_i64(p.router, p.router_dtype, phys * p.rs[0] + h * p.rs[1] + lv * p.rs[2]) ==
+              load_any_i64(p.qrouter, p.qrouter_dtype, b * p.qrs[0] + h * p.qrs[1] + lv * p.qrs[2]);
+    }
+    if (!same) return false;
+  }
   return true;
 }
 

@@ -61,7 +61,8 @@ int64_t pd_bytes(int64_t B, int64_t H, int64_t D, const PdSplit& s) {
   return B * H * (int64_t)(s.sp + s.so) * (D + 2) * 4;
 }
 
-// NI: float4 output columns per thread, D <= 32 NI.
+// NI: float4 output columns per thread, D <= 32 NI.  Registers are held to what five CTAs per SM leave (three
+// above 128 columns, whose K and V take the shared memory): all of a small batch's CTAs run at once.
 template <typename T, int NI>
 __global__ void __launch_bounds__(kPdThreads, NI <= 4 ? 5 : 3) prefix_split_kernel(const PrefixParams p, const PdSplit s, float* part) {
   extern __shared__ float sm[];

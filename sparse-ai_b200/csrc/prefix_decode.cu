@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kPdThreads, NI <= 4 ? 5 : 3) prefix_split_kern
       if (see[u] && p.r > 0) {
         if (lp != last_lp) {
           last_lp = lp;
-          last_on = page_attended(p, b, h, (own ? pre_pages : 0) + lp, n_pages, phys);
+          last_on = page_attended<4>(p, b, h, (own ? pre_pages : 0) + lp, n_pages, phys);
         }
         see[u] = last_on;
       }

@@ -44,17 +44,21 @@ __device__ __forceinline__ int64_t own_tokens(const PrefixParams& p, int64_t b) 
   return max((int64_t)0, min((int64_t)p.ctx[b], p.L * p.page));
 }
 
-// Whether head h of request b attends logical page l (of n), held in physical page phys.
+// Whether head h of request b attends logical page l (of n), held in physical page phys: kLevels levels
+// in flight.  (The join, which needs it only for rows that are computed again, takes 1: more code there
+// costs every call 2 us.)
+template <int kLevels>
 __device__ __forceinline__ bool page_attended(const PrefixParams& p, int64_t b, int64_t h, int64_t l, int64_t n,
                                               int64_t phys) {
   if ((p.sink && l == 0) || l >= n - p.local_blocks) return true;
-  for (int64_t i = 0; i < p.r; i += 4) {  // 4 levels in flight; those past r repeat the last
+#pragma unroll 1
+  for (int64_t i0 = 0; i0 < p.r; i0 += kLevels) {  // those past r repeat the last
     bool same = true;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t lv = min(i + k, p.r - 1);
-      same &= load_any_i64(p.router, p.router_dtype, phys * p.rs[0] + h * p.rs[1] + lv * p.rs[2]) ==
-              load_any_i64(p.qrouter, p.qrouter_dtype, b * p.qrs[0] + h * p.qrs[1] + lv * p.qrs[2]);
+    for (int k = 0; k < kLevels; ++k) {
+      const int64_t i = min(i0 + k, p.r - 1);
+      same &= load_any_i64(p.router, p.router_dtype, phys * p.rs[0] + h * p.rs[1] + i * p.rs[2]) ==
+              load_any_i64(p.qrouter, p.qrouter_dtype, b * p.qrs[0] + h * p.qrs[1] + i * p.qrs[2]);
     }
     if (!same) return false;
   }

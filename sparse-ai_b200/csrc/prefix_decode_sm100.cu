@@ -1428,7 +1428,7 @@ __device__ __noinline__ void exact_row(const PrefixParams& p, int64_t b, int64_t
   for (int i = 0; i < 4; ++i) qv[i] = lane + 32 * i < p.D ? to_f32<T>(q[lane + 32 * i]) * scale2 : 0.f;
   for (int64_t pg = 0; pg < n; ++pg) {
     const int64_t phys = pg < pp ? p.ppages[pg] : p.bt[b * p.bts[0] + (pg - pp) * p.bts[1]];
-    if (phys < 0 || phys >= p.num_pages || !page_attended(p, b, h, pg, n, phys)) continue;
+    if (phys < 0 || phys >= p.num_pages || !page_attended<1>(p, b, h, pg, n, phys)) continue;
     const int64_t valid = min(p.page, pg < pp ? ptok - pg * p.page : otok - (pg - pp) * p.page);
     for (int64_t t = 0; t < valid; ++t) {
       const T* k = static_cast<const T*>(p.kc) + phys * p.ks[0] + g * p.ks[1] + t * p.ks[2];

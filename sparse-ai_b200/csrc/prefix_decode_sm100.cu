@@ -1120,12 +1120,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
             tmem_wait_st();
           }
         }
-        // P^T: a row's 128 keys as two 128-byte swizzled rows of 64, in the unused part of a Q buffer
+        // P^T: a row's 128 keys as two 128-byte swizzled rows of 64, in the unused part of a Q buffer.  A
+        // reference of -inf (no attended score yet, or none that is a number) is taken as 0: masked
+        // keys still get exp2(-inf) = 0, and an attended NaN reaches the sum and the result.
         unsigned char* pt = sm + L::kQ + grp * L::kTile + kThinP + (rl >> 6) * (kThin * 128) + (rl & 7) * 2;
         const int unit = (rl & 63) >> 3;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          const float e = ref[r] == -INFINITY ? 0.f : fast_exp2(x[r] - ref[r]);
+          const float e = fast_exp2(x[r] - (ref[r] == -INFINITY ? 0.f : ref[r]));
           sum[r] += e;
           *reinterpret_cast<uint16_t*>(pt + r * 128 + ((unit ^ (r & 7)) << 4)) = (uint16_t)pack2(e, 0.f, BF16);
         }

@@ -415,8 +415,10 @@ SA_API int64_t sa_ultrametric_prefix_decode_workspace_bytes(int dtype, int64_t B
  * are skipped (status bit 2).  A row with nothing to attend gets zeros and lse = -inf.
  *
  * dtype             SA_BF16, SA_F16 (tcgen05 path where D % 8 == 0, D <= 128, page_size % 8 == 0,
- *                   H / Hkv <= 128, H <= 256, and every row of q and the caches is 16-byte aligned
- *                   with no stride of 0) or SA_F32; D <= 256.
+ *                   H / Hkv <= 128, H <= 256, every row of q and the caches is 16-byte aligned
+ *                   with no stride of 0, and B * Hkv * max_logical_pages * page_size stays below
+ *                   about 1.8e10 where page_size divides 128 or is a multiple of it) or SA_F32;
+ *                   D <= 256.
  * q, out            (B, H, D); k_cache, v_cache (P, Hkv, page_size, D); D contiguous.
  * prefix_pages      (max_prefix_pages,) int32; block_tables (B, max_logical_pages) int32.
  * router            (P, H, TD), q_router (B, H, TD): SA_I32 or SA_I64 (not read at req_depth 0).

@@ -66,7 +66,8 @@ __device__ __forceinline__ bool page_attended(const PrefixParams& p, int64_t b, 
 }
 
 // Tensor-core path: bf16/fp16, D % 8 == 0 and <= 128, page % 8 == 0, <= 128 query heads per KV
-// head and <= 256 in all (prefix_fast_shape), and 16-byte aligned rows (prefix_fast_eligible).
+// head and <= 256 in all (prefix_fast_shape), 16-byte aligned rows, and page lists whose tiles
+// can be counted in 32 bits (prefix_fast_eligible).
 bool prefix_fast_shape(int dtype, int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page);
 bool prefix_fast_eligible(const PrefixParams& p, int dtype);
 int64_t prefix_fast_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t page, int64_t Lp, int64_t L);

@@ -1578,14 +1578,24 @@ int64_t prefix_fast_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t D
   return (int64_t)carve(nullptr, make_split(B, H / Hkv, Hkv, page, Lp, L, D), nullptr);
 }
 
+// Key tiles, weighted lengths of the line of work and tasks of the mask kernel are 32-bit numbers on the
+// device.  The host knows the widths of the page lists, not the lengths: with every page in use, the
+// tiles at their highest weights (make_line) have to stay below 2^31 and the tasks below 2^30 (a
+// task index runs past the last by less than the grid).  Weighted tiles reach that at about
+// 18 billion own tokens x KV heads over all requests: 256 requests of 8 heads, tables for 8.9
+// million tokens each.
+static bool counts_fit(const Split& s) {
+  auto tiles = [&](int64_t pages) { return (double)((pages + s.ppt - 1) / s.ppt) * s.sub; };
+  const double weight = tiles(s.Lp) * ((double)s.units[0] * (kCostPair + 2 * kCostItem) + (double)s.units[1] * (kCostOne + kCostItem)) +
+                        tiles(s.L) * s.B * s.Hkv * (kCostOne + kCostItem);
+  const double tasks = 4.0 * s.Hkv * s.row_tiles * prefix_chunks(s) + (double)s.B * own_chunks(s);
+  return weight < 2147483648.0 && tasks < 1073741824.0;
+}
+
 bool prefix_fast_eligible(const PrefixParams& p, int dtype) {
   if (!prefix_fast_shape(dtype, p.B, p.H, p.Hkv, p.D, p.page)) return false;
   if (p.num_pages < 1 || p.num_pages > INT32_MAX) return false;
-  // weighted key tiles of the whole batch stay below 2^31
-  const int64_t span = std::max<int64_t>(8, std::min<int64_t>(p.page, kT));
-  if ((double)p.B * p.Hkv * (p.L + 1) * (p.page / span + 1) * 32 > 1e9 ||
-      (double)p.B * p.Hkv * (p.Lp + 1) * (p.page / span + 1) * 32 > 1e9)
-    return false;
+  if (!counts_fit(make_split(p.B, p.G, p.Hkv, p.page, p.Lp, p.L, p.D))) return false;
   if (reinterpret_cast<uintptr_t>(p.q) % 16 || reinterpret_cast<uintptr_t>(p.kc) % 16 ||
       reinterpret_cast<uintptr_t>(p.vc) % 16)
     return false;

@@ -63,7 +63,8 @@ def ultrametric_prefix_decode(
     Returns (B, H, D) in q.dtype, and with ``return_lse`` the (B, H) fp32 natural-log LSE; a row
     that attends nothing gets zeros and -inf.  fp32, fp16 or bf16; head_dim up to 256.
     fp16/bf16 with head_dim a multiple of 8 up to 128 and a page size that is a multiple of 8 run
-    on the tensor cores, the rest on the CUDA cores."""
+    on the tensor cores, the rest on the CUDA cores, as do tables wider than about 1.8e10 tokens x KV
+    heads over all requests."""
     if q.dim() != 3:
         raise ValueError(f"q must be (B, H, D), got {tuple(q.shape)}")
     B, H, D = q.shape

@@ -34,7 +34,7 @@ class SharedPrefixCache:
     def __init__(self, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, num_heads: int,
                  tree_depth: int, max_requests: int, max_pages_per_request: int, max_prefix_pages: int,
                  num_layers: int = 1, dtype=torch.bfloat16, device="cuda"):
-        self.page_size, self.num_layers = int(page_size), int(num_layers)
+        self.page_size, self.num_layers, self.num_pages = int(page_size), int(num_layers), int(num_pages)
         shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
         self.k_cache = torch.zeros(shape, dtype=dtype, device=device)
         self.v_cache = torch.zeros(shape, dtype=dtype, device=device)
@@ -47,6 +47,7 @@ class SharedPrefixCache:
         self.prefix_table = torch.zeros((1, max_prefix_pages), **i32)
         self.prefix_len = torch.zeros(1, **i32)  # read by the decode on the device
         self._prefix_tokens = 0                  # the same number for positions
+        self._planned = False                    # requests may hold pages
 
     @property
     def prefix_tokens(self) -> int:
@@ -54,11 +55,17 @@ class SharedPrefixCache:
 
     def plan_prefix(self, num_tokens: int) -> PagedTables:
         """Pages for a prefix of ``num_tokens``; its K/V rows are then written, layer by layer, with
-        ``write``.  The cache holds one prefix, set before any request."""
+        ``write``.  The cache holds one prefix, set before any request: the positions of a request's
+        tokens count from its end, and the whole pool is free for it."""
         if self._prefix_tokens:
             raise ValueError("the cache already holds a prefix")
+        if self._planned:
+            raise ValueError("the prefix must be set before any request is planned")
         if not 0 < num_tokens <= self.prefix_table.shape[1] * self.page_size:
             raise ValueError(f"a prefix of {num_tokens} tokens does not fit {self.prefix_table.shape[1]} pages of "
+                             f"{self.page_size}")
+        if num_tokens > self.num_pages * self.page_size:
+            raise ValueError(f"a prefix of {num_tokens} tokens does not fit the cache's {self.num_pages} pages of "
                              f"{self.page_size}")
         n = torch.full((1,), int(num_tokens), dtype=torch.int32, device=self.prefix_len.device)
         t = build_paged_tables(self.prefix_len, n, self.prefix_table, self.free_pages, self.num_free,
@@ -74,6 +81,7 @@ class SharedPrefixCache:
         prefix's end."""
         t = build_paged_tables(self.context_lens, new_lens, self.block_tables, self.free_pages, self.num_free,
                                page_size=self.page_size, num_tokens=num_tokens, position_base=self._prefix_tokens)
+        self._planned = True
         self.context_lens.copy_(t.context_lens)
         self.num_free.copy_(t.num_free)
         return t

@@ -179,6 +179,25 @@ def require_cuda(name: str, *tensors) -> None:
                                f"{t.device}. There is no CPU fallback.")
 
 
+# the current device's index, without building a Device object or checking for initialisation
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def require_one_device(name: str, first: torch.Tensor, *rest) -> None:
+    """``require_cuda``, and the tensors lie on one device, the current one: the library launches on the
+    current device, with its status word and its number of SMs, and takes addresses as they are."""
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            require_cuda(name, first, *rest)
+            raise ValueError(f"{name}: the tensors must lie on one device; got cuda:{dev} and cuda:{t.get_device()}")
+    if dev < 0:
+        require_cuda(name, first)
+    if dev != current_device():
+        raise ValueError(f"{name}: the tensors lie on cuda:{dev} but the current device is cuda:{current_device()}; "
+                         f"make theirs current (torch.cuda.device)")
+
+
 def read_device_status(reset: bool = True) -> int:
     v = ctypes.c_uint(0)
     check(lib().sa_read_device_status(int(reset), ctypes.byref(v)), "sa_read_device_status")

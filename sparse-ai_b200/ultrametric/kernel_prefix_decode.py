@@ -64,7 +64,7 @@ def ultrametric_prefix_decode(
     that attends nothing gets zeros and -inf.  fp32, fp16 or bf16; head_dim up to 256.
     fp16/bf16 with head_dim a multiple of 8 up to 128 and a page size that is a multiple of 8 run
     on the tensor cores, the rest on the CUDA cores, as do tables wider than about 1.8e10 tokens x KV
-    heads over all requests."""
+    heads over all requests.  All tensors lie on the current device."""
     if q.dim() != 3:
         raise ValueError(f"q must be (B, H, D), got {tuple(q.shape)}")
     B, H, D = q.shape
@@ -100,8 +100,8 @@ def ultrametric_prefix_decode(
         plen = int(prefix_len)
         if not 0 <= plen <= Lp * page:
             raise ValueError(f"prefix_len {plen} does not fit {Lp} pages of {page}")
-    nat.require_cuda("ultrametric_prefix_decode", q, k_cache, v_cache, prefix_pages, plen_dev, block_tables,
-                     context_lens, router_indices, q_router_indices)
+    nat.require_one_device("ultrametric_prefix_decode", q, k_cache, v_cache, prefix_pages, plen_dev, block_tables,
+                           context_lens, router_indices, q_router_indices)
     code = nat.float_code(dtype)
     i32, i64 = torch.int32, torch.int64
     pp = (prefix_pages if prefix_pages.dtype is i32 else prefix_pages.to(i32)).contiguous()

@@ -13,7 +13,7 @@ CUDA graph:
   vectors) into the cache by the slot map.
 
 sparse-ai has no counterpart: its paged decode (``src/ultrametric/kernel_decode.py:188-247``)
-reads such a cache and nothing there writes one.  CUDA tensors only.
+reads such a cache and nothing there writes one.  CUDA tensors of the current device only.
 """
 
 from __future__ import annotations
@@ -99,7 +99,7 @@ def build_paged_tables(
         raise ValueError(f"num_tokens must be >= 0, got {num_tokens}")
     if position_base < 0:
         raise ValueError(f"position_base must be >= 0, got {position_base}")
-    nat.require_cuda("build_paged_tables", context_lens, new_lens, block_tables, free_pages, num_free)
+    nat.require_one_device("build_paged_tables", context_lens, new_lens, block_tables, free_pages, num_free)
     ctx, new = context_lens.contiguous(), new_lens.contiguous()
     slots = ctx.new_empty(T, dtype=torch.int64)
     # the int32 results share one allocation, those by token on 16-byte boundaries
@@ -131,7 +131,7 @@ def release_paged_requests(
     page_size = int(page_size)
     B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size,
                         ("finished", finished, torch.bool))
-    nat.require_cuda("release_paged_requests", finished, context_lens, block_tables, free_pages, num_free)
+    nat.require_one_device("release_paged_requests", finished, context_lens, block_tables, free_pages, num_free)
     ctx, done = context_lens.contiguous(), finished.contiguous()
     out_ctx, out_free = torch.empty_like(ctx), ctx.new_empty(1)
     nat.check(nat.lib().sa_paged_release(
@@ -183,7 +183,7 @@ def paged_kv_write(
     kst, vst, kcs, vcs = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
     if kcs[3] != 1 or vcs[3] != 1:
         raise ValueError("the caches' head_dim must be contiguous")
-    nat.require_cuda("paged_kv_write", k, v, slot_mapping, k_cache, v_cache, routes, router_indices)
+    nat.require_one_device("paged_kv_write", k, v, slot_mapping, k_cache, v_cache, routes, router_indices)
     code = nat.float_code(dtype)
     kk = k if kst[2] == 1 else k.contiguous()
     vv = v if vst[2] == 1 else v.contiguous()

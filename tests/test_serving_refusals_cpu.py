@@ -13,6 +13,51 @@ def _i32(*shape):
     return torch.zeros(*shape, dtype=torch.int32)
 
 
+class OnDevice(torch.Tensor):
+    """A host tensor that says it lies on a GPU."""
+
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return self.index
+
+
+def on(index, t):
+    t = t.as_subclass(OnDevice)
+    t.index = index
+    return t
+
+
+def _calls(a, b):
+    """The four operators with their first tensor on GPU a and the others on GPU b."""
+    k, c = torch.zeros(5, 2, 8), torch.zeros(3, 2, 4, 8)
+    return {
+        "build_paged_tables": lambda: build_paged_tables(
+            on(a, _i32(3)), on(b, _i32(3)), on(b, _i32(3, 4)), on(b, _i32(9)), on(b, _i32(1)), page_size=4, num_tokens=2),
+        "release_paged_requests": lambda: release_paged_requests(
+            on(a, torch.zeros(3, dtype=torch.bool)), on(b, _i32(3)), on(b, _i32(3, 4)), on(b, _i32(9)), on(b, _i32(1)),
+            page_size=4),
+        "paged_kv_write": lambda: paged_kv_write(on(a, k), on(b, k), on(b, torch.zeros(5, dtype=torch.int64)), on(b, c),
+                                                 on(b, c)),
+        "ultrametric_prefix_decode": lambda: ultrametric_prefix_decode(
+            on(a, torch.zeros(2, 4, 8)), on(b, c), on(b, c), on(b, _i32(2)), on(b, _i32(1)), on(b, _i32(2, 3)),
+            on(b, _i32(2)), on(b, _i32(3, 4, 2)), on(b, _i32(2, 4, 2)), 1),
+    }
+
+
+@pytest.mark.parametrize("name", list(_calls(0, 0)))
+def test_tensors_of_another_device(name, monkeypatch):
+    def no_launch(*a):
+        raise AssertionError("the library was called")
+    monkeypatch.setattr(nat, "lib", no_launch)
+    monkeypatch.setattr(nat, "current_device", lambda: 0)
+    for a, b in ((0, 1), (1, 0)):
+        with pytest.raises(ValueError, match="one device"):
+            _calls(a, b)[name]()
+    with pytest.raises(ValueError, match="current device"):
+        _calls(1, 1)[name]()
+
+
 def test_prefix_beyond_the_pool():
     cache = SharedPrefixCache(2, 1, 16, 8, 1, 1, 2, 2, 8, device="cpu")
     for n in (33, 100):

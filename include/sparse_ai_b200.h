@@ -382,7 +382,7 @@ SA_API int sa_paged_release(int64_t B, int64_t max_logical_pages, int64_t page_s
  * are skipped; slots past the cache are skipped with status bit 2.  When routes (T, H, TD) is
  * given, router (P, H, TD) of a page <- routes of the last row with a slot in it, which is what one
  * sa_paged_kv_append per token would leave.  Slots must be distinct and, with routes, the rows of a
- * page stand together (rows without a slot between them aside).
+ * page stand together (skipped rows between them aside).
  * dtype SA_F32 / SA_F16 / SA_BF16, D contiguous, any other stride; routes/router int32 or int64.
  */
 SA_API int sa_paged_kv_write(int dtype, int64_t T, int64_t Hkv, int64_t D, int64_t page_size,

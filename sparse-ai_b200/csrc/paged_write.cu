@@ -98,22 +98,25 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const WriteP
   if (!p.routes) return;
   // Routing vectors, one warp per token: a page takes that of the last of its rows, i.e. of a row whose
   // next row with a slot is in another page.  Rows without one are passed over: 32 at first, then 512
-  // at a time (a batch padded to a fixed size ends in thousands of them).
+  // at a time (a batch padded to a fixed size ends in thousands of them).  So are those whose slot lies
+  // past the cache: taken for another page's, they would leave a page with two last rows, and two
+  // warps writing its vector.
   const int lane = tid & 31;
+  const uint64_t slots_end = (uint64_t)(p.num_pages * p.page);
   const bool all = tokens == 1;  // the CTA's warps share its only token
   for (int j = all ? 0 : tid >> 5; j < tokens; j += all ? 1 : kWriteThreads / 32) {
     const int64_t t = t0 + j, page = s_page[j];
     if (page < 0) continue;
     int64_t n0 = t + 1, first = -1;  // the next slot
     int64_t next = n0 + lane < p.T ? p.slots[n0 + lane] : -1;
-    unsigned has = __ballot_sync(0xffffffffu, next >= 0);
+    unsigned has = __ballot_sync(0xffffffffu, (uint64_t)next < slots_end);
     if (has) first = __shfl_sync(0xffffffffu, next, __ffs(has) - 1);
 #pragma unroll 1
     for (n0 += 32; !has && n0 < p.T; n0 += 32 * 16) {
       unsigned found = 0;  // bit k: row n0 + 32 k + lane has a slot
 #pragma unroll
       for (int k = 0; k < 16; ++k)
-        found |= n0 + 32 * k + lane < p.T && p.slots[n0 + 32 * k + lane] >= 0 ? 1u << k : 0u;
+        found |= n0 + 32 * k + lane < p.T && (uint64_t)p.slots[n0 + 32 * k + lane] < slots_end ? 1u << k : 0u;
       const unsigned any = __reduce_or_sync(0xffffffffu, found);
       if (!any) continue;
       const int k = __ffs(any) - 1;

@@ -15,6 +15,27 @@ def _i32(x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
 
+@pytest.mark.parametrize("T", [40, 3000])
+def test_write_takes_routes_across_slots_past_the_cache(T):
+    """A row whose slot lies past the cache is skipped, also between the rows of one page."""
+    torch.manual_seed(T)
+    Hkv, D, page, H, TD = 2, 64, 16, 4, 3
+    P = -(-T // page)
+    slots = torch.arange(T, device=DEV)
+    gone = torch.rand(T, device=DEV) < 0.4
+    slots = torch.where(gone, P * page + slots, slots)
+    k, v = torch.randn(T, Hkv, D, device=DEV), torch.randn(T, Hkv, D, device=DEV)
+    kc, vc = torch.zeros(P, Hkv, page, D, device=DEV), torch.zeros(P, Hkv, page, D, device=DEV)
+    routes = torch.randint(0, 1000, (T, H, TD), device=DEV, dtype=torch.int32)
+    router = torch.full((P, H, TD), -1, dtype=torch.int32, device=DEV)
+    want = [x.cpu().clone() for x in (kc, vc, router)]
+    so.write_rows(k.cpu(), v.cpu(), slots.cpu(), want[0], want[1], routes.cpu(), want[2])
+    for _ in range(5):
+        paged_kv_write(k, v, slots, kc, vc, routes=routes, router_indices=router)
+        assert torch.equal(kc.cpu(), want[0]) and torch.equal(vc.cpu(), want[1]) and torch.equal(router.cpu(), want[2])
+    assert nat.read_device_status(reset=True) == 2
+
+
 def test_prefix_is_set_before_any_request():
     cache = SharedPrefixCache(8, 1, 16, 64, 1, 1, 2, 4, 4, device=DEV)
     cache.plan(_i32([3, 0]), 3)

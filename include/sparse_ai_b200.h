@@ -342,14 +342,16 @@ SA_API int sa_paged_kv_append(int dtype, int64_t B, int64_t Hkv, int64_t D, int6
  * page_size) - ceil(ctx / page_size) pages more, taken in request order from the top of the stack
  * free_pages[0, num_free): the k-th page taken is free_pages[num_free - 1 - k].  A request is
  * refused (status bit 2, nothing of it changes, its rows get slot -1) when a length is negative, its
- * pages exceed max_logical_pages, its rows exceed num_tokens, or it needs pages and the running
- * sum of pages needed, refused-for-pages requests included, exceeds num_free.
+ * new length or last position exceeds 2^31 - 1, its pages exceed max_logical_pages, its rows exceed
+ * num_tokens, or it needs pages and the running sum of pages needed, refused-for-pages requests
+ * included, exceeds num_free.
  *
  * block_tables      (B, max_logical_pages) int32 with bt_strides, in place: new entries only.
  * slot_mapping      (num_tokens,) int64 out: page * page_size + row in the page, -1 for refused
  *                   requests' rows and rows past cu[B].
  * request_ids       (num_tokens,) int32 out (-1 past cu[B]); positions (num_tokens,) int32 out:
- *                   position_base + the token's position in its request (0 past cu[B]).
+ *                   position_base + the token's position in its request, at most 2^31 - 1 (0 past
+ *                   cu[B]).
  * cu_new_lens       (B + 1,) int32 out.
  * context_lens_out  (B,) int32 out; num_free_out (1,) int32 out: must not alias the inputs, so a
  *                   call can be repeated.

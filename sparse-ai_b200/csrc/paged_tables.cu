@@ -84,7 +84,9 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesP
     run_rows += tot;
     const int64_t old_pages = (max(c, (int64_t)0) + p.page - 1) / p.page;
     const int64_t all_pages = (max(c, (int64_t)0) + max(n, (int64_t)0) + p.page - 1) / p.page;
-    const bool ok = in && c >= 0 && n >= 0 && all_pages <= p.L && end <= p.rows && c + n <= INT32_MAX;
+    // lengths and positions are 32-bit numbers
+    const bool ok = in && c >= 0 && n >= 0 && all_pages <= p.L && end <= p.rows && c + n <= INT32_MAX &&
+                    (n == 0 || p.pos_base + c + n - 1 <= INT32_MAX);
     const int64_t need = ok ? all_pages - old_pages : 0;
     const int64_t incl = run_need + cta_incl_sum(need, s_warp, &tot);
     run_need += tot;
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesP
       while (s_cu[lo + 1] <= t) ++lo;
       const int64_t c = p.ctx[lo], ps = max(c, (int64_t)0) + (t - s_cu[lo]);
       rid[i] = lo;
-      pos[i] = (int32_t)(p.pos_base + ps);
+      pos[i] = (int32_t)min(p.pos_base + ps, (int64_t)INT32_MAX);  // past it: a refused request's rows
       const int first = s_first[lo];
       if (first < 0) continue;
       const int64_t lp = ps / p.page, off = ps - lp * p.page, old_pages = (c + p.page - 1) / p.page;

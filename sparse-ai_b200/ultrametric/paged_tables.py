@@ -88,9 +88,10 @@ def build_paged_tables(
                             or more to keep one shape from step to step).
     position_base           added to the positions (the length of a shared prefix).
 
-    A request that does not fit (negative length, more than L pages, rows past ``num_tokens``, or
-    no pages left) is refused: its rows get slot -1, its length and table stay, and the device
-    status gets bit 2.  Requests after one that found no pages are refused too if they need any.
+    A request that does not fit (negative length, more than L pages, rows past ``num_tokens``,
+    positions past 2^31 - 1, or no pages left) is refused: its rows get slot -1, its length and
+    table stay, and the device status gets bit 2.  Requests after one that found no pages are
+    refused too if they need any.
     Nothing is read back to the host."""
     page_size, T, position_base = int(page_size), int(num_tokens), int(position_base)
     B, L = _tables_args(context_lens, block_tables, free_pages, num_free, page_size,

@@ -15,6 +15,25 @@ def _i32(x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
 
+def test_positions_stay_in_32_bits():
+    top = 2 ** 31 - 1
+
+    def build(ctx, new, base):
+        bt = torch.full((len(ctx), 4), -7, dtype=torch.int32, device=DEV)
+        t = build_paged_tables(_i32(ctx), _i32(new), bt, _i32(list(range(20))), _i32([20]), page_size=16,
+                               num_tokens=sum(new), position_base=base)
+        assert t.positions.min() >= 0
+        return t, nat.read_device_status(reset=True)
+    # the last position is the largest that 32 bits hold
+    t, status = build([0, 5, 0], [3, 0, 6], top - 5)
+    assert status == 0 and t.positions.tolist() == [top - 5 + i for i in (0, 1, 2, 0, 1, 2, 3, 4, 5)]
+    assert t.context_lens.tolist() == [3, 5, 6] and t.slot_mapping.ge(0).all()
+    # one more is refused, like any request that does not fit; idle requests are not
+    t, status = build([0, 5, 0, 16], [3, 0, 7, 0], top - 5)
+    assert status == 2 and t.context_lens.tolist() == [3, 5, 0, 16] and t.num_free.tolist() == [19]
+    assert t.slot_mapping[:3].ge(0).all() and t.slot_mapping[3:].eq(-1).all()
+
+
 @pytest.mark.parametrize("T", [40, 3000])
 def test_write_takes_routes_across_slots_past_the_cache(T):
     """A row whose slot lies past the cache is skipped, also between the rows of one page."""

@@ -415,7 +415,7 @@ int sa_ultrametric_prefix_decode(int dtype, int64_t B, int64_t H, int64_t Hkv, i
   if (B == 0) return SA_OK;
   if (!q || !q_strides || !k_strides || !v_strides || (num_pages && (!k_cache || !v_cache)) ||
       (max_prefix_pages && !prefix_pages) || (max_logical_pages && !block_tables) || !bt_strides || !context_lens ||
-      !router_strides || !q_router_strides || (req_depth && (!router || !q_router)) || !out || !out_strides)
+      !router_strides || !q_router_strides || (req_depth && ((num_pages && !router) || !q_router)) || !out || !out_strides)
     return fail(SA_EINVAL, "prefix decode: null pointer argument");
   if (q_strides[2] != 1 || k_strides[3] != 1 || v_strides[3] != 1 || out_strides[2] != 1)
     return fail(SA_EUNSUPPORTED, "prefix decode: head_dim must be the contiguous dimension");

@@ -50,3 +50,12 @@ def test_both_sides_of_the_limit(width, fast, depth):
     got, tensor = run(t, n, depth, 1, False)
     assert tensor == fast
     check(t, n, depth, 1, False, got=got)
+
+
+def test_a_cache_without_pages():
+    t, _ = make(3, 4, 2, 64, 16, 0, [0, 0, 0], seed=1)
+    for key in ("kc", "vc", "ri"):
+        t[key] = t[key][:0].contiguous()
+    for depth in (0, 1):
+        out, lse = call(t, 0, depth, 1, True)
+        assert (out == 0).all() and torch.isneginf(lse).all()

@@ -44,6 +44,14 @@ class PagedTables(NamedTuple):
     num_free: torch.Tensor
 
 
+def _check_written(name, t):
+    """Refuse a broadcast tensor that the kernels write: its elements share addresses."""
+    st = t.stride()
+    if 0 in st and any(s == 0 and n > 1 for s, n in zip(st, t.shape)):
+        raise ValueError(f"{name} is written in place and must not be broadcast; got strides {tuple(st)} for "
+                         f"{tuple(t.shape)}")
+
+
 def _tables_args(context_lens, block_tables, free_pages, num_free, page_size, per_request):
     """(B, L) of checked arguments; ``per_request`` = (name, tensor, dtype) beside the lengths."""
     i32 = torch.int32
@@ -100,6 +108,7 @@ def build_paged_tables(
         raise ValueError(f"num_tokens must be >= 0, got {num_tokens}")
     if position_base < 0:
         raise ValueError(f"position_base must be >= 0, got {position_base}")
+    _check_written("block_tables", block_tables)
     nat.require_one_device("build_paged_tables", context_lens, new_lens, block_tables, free_pages, num_free)
     ctx, new = context_lens.contiguous(), new_lens.contiguous()
     slots = ctx.new_empty(T, dtype=torch.int64)
@@ -181,9 +190,12 @@ def paged_kv_write(
         if t2 != T or router_indices.shape != (P, H, TD):
             raise ValueError(f"routes must be (T, H, TD) and router_indices (num_pages, H, TD); got "
                              f"{tuple(routes.shape)}, {tuple(router_indices.shape)}")
+        _check_written("router_indices", router_indices)
     kst, vst, kcs, vcs = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
     if kcs[3] != 1 or vcs[3] != 1:
         raise ValueError("the caches' head_dim must be contiguous")
+    _check_written("k_cache", k_cache)
+    _check_written("v_cache", v_cache)
     nat.require_one_device("paged_kv_write", k, v, slot_mapping, k_cache, v_cache, routes, router_indices)
     code = nat.float_code(dtype)
     kk = k if kst[2] == 1 else k.contiguous()

@@ -67,3 +67,18 @@ def test_prefix_beyond_the_pool():
     with pytest.raises(RuntimeError, match="no CPU fallback"):  # fits: only the device is missing
         cache.plan_prefix(32)
     assert cache.prefix_tokens == 0
+
+
+def test_broadcast_outputs():
+    k, c, s = torch.zeros(5, 2, 8), torch.zeros(3, 2, 4, 8), torch.zeros(5, dtype=torch.int64)
+    wide = torch.zeros(3, 1, 4, 8).expand(3, 2, 4, 8)
+    routes, router = _i32(5, 4, 2), _i32(1, 4, 2).expand(3, 4, 2)
+    for args, kw in (((k, k, s, wide, c), {}), ((k, k, s, c, wide), {}),
+                     ((k, k, s, c, c), dict(routes=routes, router_indices=router))):
+        with pytest.raises(ValueError, match="written in place"):
+            paged_kv_write(*args, **kw)
+    with pytest.raises(ValueError, match="written in place"):
+        build_paged_tables(_i32(3), _i32(3), _i32(1, 4).expand(3, 4), _i32(9), _i32(1), page_size=4, num_tokens=2)
+    # a dimension of one may have any stride
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        build_paged_tables(_i32(1), _i32(1), _i32(4).as_strided((1, 4), (0, 1)), _i32(9), _i32(1), page_size=4, num_tokens=2)

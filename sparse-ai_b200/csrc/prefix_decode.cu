@@ -426,6 +426,8 @@ int sa_ultrametric_prefix_decode(int dtype, int64_t B, int64_t H, int64_t Hkv, i
   if (workspace_bytes < need || (need && !workspace))
     return fail(SA_EWORKSPACE, "prefix decode: workspace too small (" + std::to_string(workspace_bytes) + " < " +
                                    std::to_string(need) + ")");
+  if (reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(SA_EINVAL, "prefix decode: workspace must be 256-byte aligned");
   if (int rc = check_stream_device(stream, "prefix decode")) return rc;
   PrefixParams p{};
   p.B = B;

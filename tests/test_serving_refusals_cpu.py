@@ -82,3 +82,17 @@ def test_broadcast_outputs():
     # a dimension of one may have any stride
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         build_paged_tables(_i32(1), _i32(1), _i32(4).as_strided((1, 4), (0, 1)), _i32(9), _i32(1), page_size=4, num_tokens=2)
+
+
+def test_decode_workspace_alignment():
+    lib = nat.lib()
+    st, buf = (ctypes.c_int64 * 4)(1, 1, 1, 1), ctypes.create_string_buffer(4096)
+    at = -(-ctypes.addressof(buf) // 256) * 256
+
+    def decode(ws):
+        p = at
+        return lib.sa_ultrametric_prefix_decode(
+            nat.SA_F16, 2, 4, 2, 16, 4, 6, p, st, p, st, p, st, p, 2, 8, None, p, st, 3, p, p, nat.SA_I32, st, p, nat.SA_I32,
+            st, 3, 1, 0, 0, p, st, None, ws, 1 << 40, None)
+    for off in (1, 4, 16, 128):
+        assert decode(at + off) == nat.SA_EINVAL and b"256-byte aligned" in lib.sa_last_error()

@@ -427,23 +427,22 @@ __global__ void __launch_bounds__(kMaskWarps * 32) prefix_mask_kernel(const __gr
 // ---------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------
-// Warp maximum of a float, and a barrier of `threads` threads that returns the OR of a predicate.
+// Warp maximum of a float, and a barrier of `threads` threads that returns how many brought pred.
 __device__ __forceinline__ float redux_max(float x) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
   return r;
 }
-__device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t threads, bool pred) {
+__device__ __forceinline__ int named_bar_count(uint32_t id, uint32_t threads, bool pred) {
   uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
+      "barrier.cta.red.popc.u32 %0, %2, %3, p;\n\t}"
       : "=r"(r)
       : "r"((uint32_t)pred), "r"(id), "r"(threads)
       : "memory");
-  return r != 0;
+  return (int)r;
 }
 
 // 32 lanes x N consecutive 32-bit columns (N = 4, 8 or 16).
@@ -1034,6 +1033,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
     int slot = 0;
     const int my_page = rl / S.bn;  // page of this key within a tile
     float* s_max = reinterpret_cast<float*>(sm + L::kMisc + 192) + grp * 4 * kThin;  // [4 warps][kThin]
+    // The group's warps meet at a named barrier, which has no limit of its own: a warp whose wait gave
+    // up must not leave the others in it.  So a warp at the end of its role keeps meeting them until
+    // all four are there, one thread of it counted; the others, 32 threads of a warp or none, run
+    // into their own limits meanwhile.
+    auto meet = [&](bool pred) -> bool { return named_bar_count(1 + grp, kGroupThreads, pred) >= 32; };
     // V rows past the valid keys meet P = 0 in the product's last K step: they must be finite, so they
     // are cleared (in a pair tile by both groups, with the same zeros).
     auto clear_tail = [&](int vr) -> bool {
@@ -1086,7 +1090,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         tmem_wait_ld();
         // Scores in log2 units, -inf by selection where a row does not attend this key; each row's
         // maximum over the warp's keys against the shared reference.
-        bool up = false;
+        bool up = false;  // the same in all of a warp's lanes
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
           x[r] = (gm >> r) & 1u ? x[r] * sc2 : -INFINITY;
@@ -1094,7 +1098,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           up |= wm > ref[r] + kRescaleThreshold || (ref[r] == -INFINITY && wm != -INFINITY);
           if (lane == 0) s_max[quarter * kThin + r] = wm;
         }
-        if (named_bar_or(1 + grp, kGroupThreads, up)) {
+        if (meet(up)) {
           // some row's reference moves, to its maximum over the tile's keys; the sums and O^T (a row is a
           // column of it; S(i) being complete implies that the lane's last product is) follow
           float f[NR];
@@ -1108,7 +1112,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
               ref[r] = mt;
             }
           }
-          named_bar_sync(1 + grp, kGroupThreads);  // s_max is read
+          meet(false);  // s_max is read
           if (had_t) {
             float o[NR];
             uint32_t u[NR];
@@ -1162,7 +1166,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       tmem_ldn<NR>(lane_addr + col_o, o);
       tmem_wait_ld();
       tc_fence_before();
-      named_bar_sync(1 + grp, kGroupThreads);  // s_max is complete, O^T is read
+      meet(false);  // s_max is complete, O^T is read
       if (lane == 0) mbar_arrive(&bars[L::bOFree + grp]);
       float m = -INFINITY;
 #pragma unroll
@@ -1171,7 +1175,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         if (r == rl) m = ref[r];
       }
       if (rl < nrow) ml[rl] = make_float2(m, s_max[rl] + s_max[kThin + rl] + s_max[2 * kThin + rl] + s_max[3 * kThin + rl]);
-      named_bar_sync(1 + grp, kGroupThreads);  // s_max is read: the next tile may write it
+      meet(false);  // s_max is read: the next tile may write it
       return true;
     };
 
@@ -1397,6 +1401,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[L::bOFree + grp]);
       }
+    }
+    while (named_bar_count(1 + grp, kGroupThreads, lane == 0) != 4) {
     }
   }
 

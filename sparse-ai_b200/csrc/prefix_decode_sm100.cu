@@ -109,7 +109,7 @@ struct Layout {
   // barriers
   static constexpr int bFull = 0, bEmpty = bFull + kSlots, bQFull = bEmpty + kSlots, bQEmpty = bQFull + 2,
                        bSFull = bQEmpty + 2, bPFull = bSFull + 2, bODone = bPFull + 2, bOFree = bODone + 2,
-                       bDFull = bOFree + 2, bDEmpty = bDFull + kDescs, bNum = bDEmpty + kDescs;
+                       bDFull = bOFree + 2, bDEmpty = bDFull + kDescs, bDrain = bDEmpty + kDescs, bNum = bDrain + 1;
   static constexpr uint32_t kMisc = kBars + bNum * 8;  // tmem slot, scan scratch, maxima of thin items
   static constexpr uint32_t kBytes = kMisc + 192 + 2 * 4 * kThin * 4;
   static constexpr uint32_t kAlloc = kBytes + 1024 <= kMaxSmem ? kBytes + 1024 : kMaxSmem;
@@ -492,7 +492,9 @@ __device__ __forceinline__ void tmem_stn(uint32_t taddr, const uint32_t (&v)[N])
 // Bounded waits as in common.cuh, counted in tries instead of timed: half the instructions at each
 // of the kernel's dozen waits, which matters where every role's code competes for the
 // instruction cache.  A try on a phase that stays incomplete suspends the thread for about 8 k
-// cycles, so kMaxTries of them are about a second.
+// cycles, so kMaxTries of them are about a second.  A warp whose wait gives up leaves its role, and the
+// others run into their own limits; the MMA issuer ends after its products and, where it did not come
+// to the last item (so that loads may be unused), after the loads in flight, with a limit too.
 constexpr uint32_t kMaxTries = 1u << 18;
 
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigned* st) {
@@ -505,6 +507,25 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, unsigne
 }
 __device__ __forceinline__ bool wait_bar_warp(uint64_t* bar, uint32_t parity, unsigned* st) {
   return __all_sync(0xffffffffu, wait_bar(bar, parity, st));
+}
+
+// Loads in flight where the MMA issuer gave up: the ring's entries from the oldest that is not released
+// (u), then the Q buffers.  Entries released out of turn (K of tiles before k_end / 2) have passed to
+// the entry a ring's length on.  What was never issued runs into the limit.
+template <uint32_t kSlots>
+__device__ __noinline__ void settle(uint64_t* full, uint64_t* q_full, uint32_t u, uint32_t k_end, uint32_t nq) {
+  uint32_t open = (1u << (kSlots + 2)) - 1u;
+  const long long t0 = clock64();
+  while (open && clock64() - t0 < (1ll << 31)) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kSlots + 2; ++i) {
+      uint32_t e = u + i;
+      if (!(e & 1) && e < k_end) e += kSlots;
+      const uint32_t q = nq + i - kSlots;
+      if (i < kSlots ? mbar_test(full + e % kSlots, (e / kSlots) & 1) : mbar_test(q_full + (q & 1), (q >> 1) & 1))
+        open &= ~(1u << i);
+    }
+  }
 }
 
 template <int DT, bool BF16>
@@ -545,6 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       mbar_init(&bars[L::bODone + i], 1);
       mbar_init(&bars[L::bOFree + i], 4);
     }
+    mbar_init(&bars[L::bDrain], 1);
     for (int i = 0; i < L::kDescs; ++i) {
       mbar_init(&bars[L::bDFull + i], 1);
       mbar_init(&bars[L::bDEmpty + i], 3 + 8);  // two producers, MMA warp, 8 softmax warps
@@ -893,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
       int in_item = 0;          // key tiles of the item so far
       int left = 0, rts = 0;    // row tiles of the current key tile still to multiply, of how many
       int flags = 0, vr = 0, stage = 0;
-      bool flush = false;
+      bool flush = false, end = false;
       long long idle = clock64();
       // Polls what it may do next: a pending P V once its P is there (at the latest before the Q K^T
       // that reuses its lane), and meanwhile the next key tile's descriptor, Q and K, so that
@@ -962,7 +984,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           --np;
           busy = true;
         } else if (flush && np == 0) {
-          if (flags & F_END) break;
+          if ((end = flags & F_END)) break;
           flush = false;
         }
         if (stage == 3 && np < 2) {
@@ -1013,6 +1035,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_sm100_kernel(const __grid_
           raise_status(st, kStatusWaitTimeout);
           break;
         }
+      }
+      tc_commit(&bars[L::bDrain]);
+      wait_bar(&bars[L::bDrain], 0, st);
+      if (__builtin_expect(!end, 0)) {
+        settle<L::kSlots>(&bars[L::bFull], &bars[L::bQFull], np > 0 ? 2 * j0.tile + 1 : 2 * tile, 2 * tile, nq);
       }
       }
     }

@@ -47,7 +47,7 @@ PdSplit pd_split(int64_t B, int64_t H, int64_t Hkv, int64_t page, int64_t Lp, in
   s.row_tiles = (int)((B * G + kRows - 1) / kRows);
   s.own_tiles = (int)((G + kRows - 1) / kRows);
   auto splits = [](int64_t ctas, int64_t tokens) {
-    const int64_t want = (4 * 148 + ctas - 1) / std::max<int64_t>(ctas, 1);
+    const int64_t want = (4 * device_sm_count() + ctas - 1) / std::max<int64_t>(ctas, 1);
     const int64_t cap = (tokens + kKeys - 1) / kKeys;
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, cap, kMaxSplits}));
   };

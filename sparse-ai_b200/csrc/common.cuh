@@ -71,7 +71,9 @@ __device__ __forceinline__ int64_t load_any_i64(const void* p, int dtype, int64_
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Hardware base-2 exponential (MUFU.EX2); inputs are <= 8 after the max shift, -inf -> 0.
+// Hardware base-2 exponential (MUFU.EX2), -inf -> 0.  Inputs that count are at most 8 after the max
+// shift; the shared-prefix decode's one-pass tiles accept results of up to 2^13 and compute tiles
+// with larger ones, or an overflow, again.
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

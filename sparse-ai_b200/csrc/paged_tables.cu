@@ -11,7 +11,7 @@
 // two dependent sums over the requests and one page lookup per token.  So there is one launch:
 // every CTA repeats the sums over all requests in its own shared memory (B / 256 rounds of two
 // block scans) instead of waiting for a first kernel's, and then fills its share of the token rows.
-// 64 requests with a token each: 5.9 us; 256 requests with 120001 tokens (2.4 MB written): 5.8 us, all of
+// 64 requests with a token each: 5.9 us; 256 requests with 120001 tokens (2.0 MB written): 5.8 us, all of
 // it latency (launch, lengths, sums, search, page, store).
 #include <algorithm>
 #include <string>

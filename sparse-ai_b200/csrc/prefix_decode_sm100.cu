@@ -34,18 +34,22 @@
 //               the tensor pipe takes one thread's products in order;
 //   warps 0-7   two softmax warpgroups, one per lane; thread = row (thin: = key): masks by
 //               selection, running maximum (O rescaled in TMEM only when it grows by more than
-//               2^8), exp2, P to TMEM over S's columns (A operand of the next product; thin: to
-//               shared memory, B operand), partials to global memory.
+//               2^8; full prefix tiles keep the reference they find, 0 in a row's first tile,
+//               while the sums of their exponentials stay within bounds), exp2, P to TMEM over
+//               S's columns (A operand of the next product; thin: to shared memory, B operand),
+//               partials to global memory.
 // S, the sums and O are fp32; P is rounded to the cache's type, as the tensor product takes it,
 // and the sums are over the unrounded P.
 //
-// What bounds it, at 32 query and 8 KV heads of 128 bf16, pages of 64:
+// What bounds it, at 32 query and 8 KV heads of 128 bf16, pages of 64 (times of the whole decode in a CUDA
+// graph):
 //   prefix (256 requests, 32768 tokens): 141 us, 970 TFLOP/s.  A pair tile takes 4 k cycles, in which
 //     the tensor pipe works 2 k (46 % of the kernel) and the exponential unit 2 k (50 %): each lane's
 //     product -> softmax -> product chain is serial, TMEM holds no third S beside two O of 128
 //     columns, and two lanes cover each other only in part;
 //   own (64 requests, 8192 tokens each): 320 us, 6.7 TB/s, DRAM 83 % busy: HBM;
-//   both (256 requests, 32768 + up to 768): 195 us;
+//   both (256 requests, 32768 + up to 768): 195 us (222 to 232 called back to back for seconds, where
+//     the board's power limit lowers the clock);
 //   small batches: launches, a prologue of 2.8 us, one tile's latency and the join: 14 us.
 #include <algorithm>
 #include <string>
@@ -76,9 +80,14 @@ constexpr int kMaxHeadWords = 8;            // query heads <= 256 (mask kernel)
 // a tile of either other kind, and what an item costs besides its tiles (fill, drain and partial
 // states; of a pair item twice that), spread over its tiles.  With routing, own and single tiles
 // count by the share of their pages that some row attends.  Fitted by timing: 256 requests on a
-// prefix of 32768 and up to 768 own tokens take 195 us with these, 230 with 16 / 11 / 14 (the traced
-// cycles of a tile on an idle GPU: beside pair tiles, own tiles have more of HBM to themselves)
-// and 228 with 24 / 9 / 9.
+// prefix of 32768 and up to 768 own tokens take 195 us with these, 226 with 16 / 11 / 14 (the traced
+// cycles of a tile on an idle GPU: beside pair tiles, own tiles have more of HBM to themselves),
+// 228 with 24 / 9 / 9, 202 with 18 / 9 / 12, 229 with 18 / 7 / 6, 213 with 18 / 12 / 6.  Against these five, in
+// the same order, at other sizes: head_dim 64, the same lengths 172 (202, 186, 179, 186, 188); prefix
+// 8192 and 500 to 2000 own 238 (266, 247, 238, 244, 259), at head_dim 64 187 (238, 184, 187, 180, 232); 200
+// requests of 16 / 4 heads on 6000 and up to 150 39 (46, 42, 42, 40, 40); 128 requests of 16 / 16 heads of 96
+// on 5000 and up to 600 91 (98, 96, 104, 94, 87).  The worst found: 96 requests of 64 / 8 heads on 20000
+// and up to 900, 114 (111, 136, 104, 131, 107).
 constexpr int kCostPair = 18, kCostOne = 9, kCostItem = 6;
 
 enum { F_FIRST = 1, F_LAST = 2, F_EMPTY = 4, F_END = 8, F_PAIR = 16, F_OWN = 32, F_THIN = 64 };
